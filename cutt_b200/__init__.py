@@ -15,12 +15,16 @@ import ctypes
 import os
 from typing import Sequence
 
+from .rows import (CUTT_ROWS_BF16, CUTT_ROWS_BYTES, CUTT_ROWS_F16, CUTT_ROWS_F32, PagedRows, PagePlan, RowPlan,
+                   bind as _bind_rows)
+
 __all__ = [
     "CUTT_SUCCESS", "CUTT_INVALID_PLAN", "CUTT_INVALID_PARAMETER", "CUTT_INVALID_DEVICE",
     "CUTT_INTERNAL_ERROR", "CUTT_UNDEFINED_ERROR", "CuttError", "lib", "lib_path",
     "cuttPlan", "cuttPlanMeasure", "cuttExecute", "cuttDestroy", "plan_describe",
     "num_candidates", "plan_candidate", "plan_params", "transpose_host", "launch_count", "copy_timeouts", "copy_noalloc", "copy_noalloc_timeouts",
     "clear_plan_cache", "debug_force_wide", "plan_cache_save", "plan_cache_load", "plan_cache_size", "Plan",
+    "CUTT_ROWS_BYTES", "CUTT_ROWS_F16", "CUTT_ROWS_BF16", "CUTT_ROWS_F32", "RowPlan", "PagePlan", "PagedRows",
 ]
 
 # cuttResult (src/cutt.h:34-41): fixed values
@@ -112,6 +116,7 @@ def lib() -> ctypes.CDLL:
                  "cutt_c_plan_describe", "cutt_c_num_candidates", "cutt_c_plan_candidate",
                  "cutt_c_plan_params", "cutt_c_transpose_host"):
         getattr(L, name).restype = ctypes.c_int
+    _bind_rows(L)
     _lib = L
     return L
 

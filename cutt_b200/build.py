@@ -24,12 +24,16 @@ GENCODE = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-Xptxas", "-v"] + GENCODE
 CXX_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-Wall", "-Wno-unknown-pragmas"]
 
-CU_SOURCES = ["kernels.cu", "bulk_copy.cu", "small_elt.cu", "tma_transpose.cu", "tile2d.cu", "cutt.cu"]
-CXX_SOURCES = ["planner.cpp"]
+CU_SOURCES = ["kernels.cu", "bulk_copy.cu", "small_elt.cu", "tma_transpose.cu", "tile2d.cu", "cutt.cu",
+              "rows_map.cu", "rows_move.cu", "pages.cu", "rows_api.cu"]
+CXX_SOURCES = ["planner.cpp", "rows_plan.cpp"]
 HEADERS = ["permute_desc.h", "permute_tile_impl.h", "planner.h", "kernels.h", "cost_model_data.h", "rowcopy_impl.h", "small_elt_impl.h",
            "tma_transpose.h", "tile2d.h",
            os.path.join("..", "..", "include", "cutt.h"), os.path.join("..", "..", "include", "cutt_c.h"),
            os.path.join("..", "..", "include", "cutt_mg.h")]
+# row operators: their headers, and the sources that include them
+ROWS_HEADERS = ["rows.h", "rows_plan.h", os.path.join("..", "..", "include", "cutt_rows.h")]
+ROWS_SOURCES = ["rows_map.cu", "rows_move.cu", "pages.cu", "rows_api.cu", "rows_plan.cpp", "cutt.cu"]
 
 
 def _newer(target: str, deps) -> bool:
@@ -53,12 +57,16 @@ def build(force: bool = False, verbose: bool = False) -> dict:
     os.makedirs(LIBDIR, exist_ok=True)
     os.makedirs(OBJDIR, exist_ok=True)
     hdrs = [os.path.join(CSRC, h) for h in HEADERS] + [os.path.abspath(__file__)]
+    rows_hdrs = [os.path.join(CSRC, h) for h in ROWS_HEADERS]
     objs = []
+
+    def deps(src):
+        return hdrs + (rows_hdrs if src in ROWS_SOURCES else [])
     with open(os.path.join(OBJDIR, "build.log"), "a") as log:
         for src in CU_SOURCES:
             s = os.path.join(CSRC, src)
             o = os.path.join(OBJDIR, src + ".o")
-            if force or _newer(o, [s] + hdrs):
+            if force or _newer(o, [s] + deps(src)):
                 out = _run([NVCC] + NVCC_FLAGS + ["-c", s, "-o", o], log)
                 if verbose:
                     print(out)
@@ -66,7 +74,7 @@ def build(force: bool = False, verbose: bool = False) -> dict:
         for src in CXX_SOURCES:
             s = os.path.join(CSRC, src)
             o = os.path.join(OBJDIR, src + ".o")
-            if force or _newer(o, [s] + hdrs):
+            if force or _newer(o, [s] + deps(src)):
                 _run(["g++"] + CXX_FLAGS + ["-c", s, "-o", o], log)
             objs.append(o)
         so = os.path.join(LIBDIR, "libcutt.so")
@@ -78,8 +86,9 @@ def build(force: bool = False, verbose: bool = False) -> dict:
                 os.remove(ar)
             _run(["ar", "rcs", ar] + objs, log)
         hc = os.path.join(LIBDIR, "libcutt_hostcheck.so")
-        hsrc = [os.path.join(CSRC, "host_interp.cpp"), os.path.join(CSRC, "planner.cpp")]
-        if force or _newer(hc, hsrc + hdrs):
+        hsrc = [os.path.join(CSRC, "host_interp.cpp"), os.path.join(CSRC, "planner.cpp"), os.path.join(CSRC, "host_rows.cpp"),
+                os.path.join(CSRC, "rows_plan.cpp")]
+        if force or _newer(hc, hsrc + hdrs + rows_hdrs):
             _run(["g++"] + CXX_FLAGS + ["-shared", "-o", hc] + hsrc, log)
     return {"so": so, "a": ar, "hostcheck": hc}
 

@@ -27,6 +27,7 @@
 #include "kernels.h"
 #include <algorithm>
 #include "planner.h"
+#include "rows.h"
 #include "small_elt_impl.h"
 
 using namespace cuttb;
@@ -749,6 +750,7 @@ cuttResult cuttPlanMeasure(cuttHandle* handle, int rank, int* dim, int* permutat
 }
 
 cuttResult cuttDestroy(cuttHandle handle) {
+  if (handle & kRowsHandleBit) return rows_destroy(handle) ? CUTT_SUCCESS : CUTT_INVALID_PLAN;
   std::lock_guard<std::mutex> lk(g_mutex);
   auto it = g_plans.find(handle);
   if (it == g_plans.end()) return CUTT_INVALID_PLAN;
@@ -851,6 +853,10 @@ int cutt_c_execute(unsigned int handle, void* idata, void* odata) {
 int cutt_c_destroy(unsigned int handle) { return (int)cuttDestroy(handle); }
 
 int cutt_c_plan_describe(unsigned int handle, char* buf, size_t len) {
+  if (handle & kRowsHandleBit) {
+    if (!buf || !len) return CUTT_INVALID_PARAMETER;
+    return rows_describe(handle, buf, len) ? CUTT_SUCCESS : CUTT_INVALID_PLAN;
+  }
   std::lock_guard<std::mutex> lk(g_mutex);
   auto it = g_plans.find(handle);
   if (it == g_plans.end()) return CUTT_INVALID_PLAN;

@@ -1,0 +1,108 @@
+// Test-only: the argument checks and the index arithmetic of the row operators on the host.
+#include <vector>
+
+#include "rows_plan.h"
+
+using namespace cuttb;
+
+extern "C" {
+
+int cutt_hostcheck_rows_shape(int tokens, int choices, int experts, int first, int align, int capacity, int width, int type) {
+  return check_rows_shape(RowsShape{tokens, choices, experts, first, align, capacity, width, type});
+}
+
+int cutt_hostcheck_pages_shape(int requests, int pageSize, int tableWidth, int maxTokens) {
+  return check_pages_shape(PagesShape{requests, pageSize, tableWidth, maxTokens, FastDiv()});
+}
+
+int cutt_hostcheck_paged_shape(int tokens, int heads, int headSize, int elt, int pages, int pageSize, long long pageStride,
+                               long long slotStride, long long headStride) {
+  return check_paged_shape(PagedShape{tokens, heads, headSize, elt, pages, pageSize, pageStride, slotStride, headStride});
+}
+
+// The checks of a call on addresses that are never read.
+int cutt_hostcheck_rows_sort(const int* shape, const void* expertOf, size_t sizeofIndex, const void* count, const void* offset,
+                             const void* rowOf, const void* slotOf) {
+  const RowsShape s{shape[0], shape[1], shape[2], shape[3], shape[4], shape[5], shape[6], shape[7]};
+  return check_rows_sort(s, expertOf, sizeofIndex, count, offset, rowOf, slotOf);
+}
+
+int cutt_hostcheck_rows_move(const int* shape, const void* token, long long tokenStride, const void* row, long long rowStride,
+                             const void* rowOf, const void* count, const void* offset, const void* weight, const void* other,
+                             long long otherStride, const void* dweight, int rowsOut) {
+  const RowsShape s{shape[0], shape[1], shape[2], shape[3], shape[4], shape[5], shape[6], shape[7]};
+  return check_rows_move(s, RowsMoveArgs{token, tokenStride, row, rowStride, (const int*)rowOf, (const int*)count, (const int*)offset,
+                                         (const float*)weight, other, otherStride, (const float*)dweight, rowsOut != 0, rowsOut != 0});
+}
+
+int cutt_hostcheck_pages_build(const int* shape, const void* held, const void* added, const void* freeList, const void* poolIn,
+                               const void* poolOut, const void* table, long long tableStride, const void* tokenOffset,
+                               const void* pageOffset, const void* slot) {
+  const PagesShape s{shape[0], shape[1], shape[2], shape[3], FastDiv()};
+  return check_pages_build(s, held, added, freeList, poolIn, poolOut, table, tableStride, tokenOffset, pageOffset, slot);
+}
+
+int cutt_hostcheck_paged_move(const int* shape, const long long* strides, const void* k, const void* v, long long tokenStride,
+                              long long headStride, const void* slot, const void* kCache, const void* vCache, int rowsOut) {
+  const PagedShape s{shape[0], shape[1], shape[2], shape[3], shape[4], shape[5], strides[0], strides[1], strides[2]};
+  return check_paged_move(s, k, v, tokenStride, headStride, slot, kCache, vCache, rowsOut != 0);
+}
+
+// cutt_pages_build on host arrays: the scan in a loop, then the kernel's expressions per token and
+// per page.  Returns the number of accesses outside the arrays (table: requests * tableStride
+// entries, freeList: freeEntries), which are skipped.
+long long cutt_hostcheck_pages_run(int requests, int pageSize, int tableWidth, int maxTokens, const int* held, const int* added,
+                                   const int* freeList, int freeEntries, const int* poolIn, int* poolOut, int* table,
+                                   long long tableStride, int* tokenOffset, int* pageOffset, long long* slot) {
+  PagesBuild p{PagesShape{requests, pageSize, tableWidth, maxTokens, make_fastdiv(pageSize)}, held, added, freeList, poolOut,
+               table, tableStride, tokenOffset, pageOffset, slot};
+  long long tokens = 0, pages = 0, bad = 0;
+  int first = 0, limit = 0;
+  if (freeList) {
+    first = clamp_pool(poolIn[0]);
+    limit = clamp_pool(poolIn[1]);
+    pages = first;
+  }
+  for (int b = 0; b < requests; b++) {
+    tokenOffset[b] = saturate(tokens);
+    tokens += added[b] > 0 ? added[b] : 0;
+    if (freeList) {
+      pageOffset[b] = (int)pages;
+      pages += pages_taken(held[b], added[b], pageSize, tableWidth);
+    }
+  }
+  tokenOffset[requests] = saturate(tokens);
+  if (freeList) {
+    if (pages > 0x7fffffffLL) bad++;
+    pageOffset[requests] = (int)pages;
+    poolOut[0] = (int)pages < (first > limit ? first : limit) ? (int)pages : (first > limit ? first : limit);
+    poolOut[1] = poolIn[1];
+    if (limit > freeEntries) return -1;
+  }
+  for (int q = 0; q < maxTokens; q++) {
+    slot[q] = -1;
+    if (q >= tokenOffset[requests]) continue;
+    const int b = last_at_or_before(tokenOffset, requests + 1, q);
+    if (b < 0 || b >= requests) { bad++; continue; }
+    slot[q] = slot_of_token(p, b, q, limit);
+  }
+  if (freeList)
+    for (int f = pageOffset[0]; f < pageOffset[requests]; f++) {
+      const int b = last_at_or_before(pageOffset, requests + 1, f);
+      if (b < 0 || b >= requests) { bad++; continue; }
+      const long long idx = pages_of(held[b] > 0 ? held[b] : 0, pageSize) + (long long)(f - pageOffset[b]);
+      if (idx >= tableWidth) { bad++; continue; }
+      take_page(p, b, f, limit);
+    }
+  return bad;
+}
+
+// Element offset of a slot in a cache, -1 where it is not one of the cache's.
+long long cutt_hostcheck_cache_offset(int pages, int pageSize, long long pageStride, long long slotStride, long long slot) {
+  const PagedShape s{1, 1, 1, 1, pages, pageSize, pageStride, slotStride, 1};
+  return cache_offset(s, slot, make_fastdiv(pageSize));
+}
+
+int cutt_hostcheck_local_expert(long long e, int first, int experts) { return local_expert(e, first, experts); }
+
+}  // extern "C"

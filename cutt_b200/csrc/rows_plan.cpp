@@ -1,0 +1,136 @@
+// Argument checks of the row operators (no CUDA calls).
+#include "rows_plan.h"
+
+namespace cuttb {
+
+namespace {
+constexpr int kBad = 2;   // CUTT_INVALID_PARAMETER
+
+bool aligned(const void* p, size_t n) { return (uintptr_t)p % n == 0; }
+}  // namespace
+
+int rows_element_bytes(int type) {
+  switch (type) {
+    case 0: return 1;
+    case 1: case 2: return 2;
+    case 3: return 4;
+  }
+  return 0;
+}
+
+int check_rows_shape(const RowsShape& s) {
+  if (!rows_element_bytes(s.type)) return kBad;
+  if (s.tokens < 0 || s.choices < 1 || (long long)s.tokens * s.choices > kRowsMaxCount) return kBad;
+  if (s.experts < 1 || s.experts > kRowsMaxExperts) return kBad;
+  if (s.first < 0 || (long long)s.first + s.experts > 0x7fffffffLL) return kBad;
+  if (s.align < 1 || s.align > kRowsMaxAlign) return kBad;
+  if (s.capacity < 1 || s.capacity > kRowsMaxCount) return kBad;
+  if (s.width < 1 || s.width > kRowsMaxWidth) return kBad;
+  return 0;
+}
+
+int check_pages_shape(const PagesShape& s) {
+  if (s.requests < 1 || s.pageSize < 1 || s.tableWidth < 1) return kBad;
+  if (s.pageSize > kRowsMaxCount || (long long)s.requests * s.tableWidth >= kRowsMaxCount) return kBad;
+  if (s.maxTokens < 0 || s.maxTokens > kRowsMaxCount) return kBad;
+  return 0;
+}
+
+int check_paged_shape(const PagedShape& s) {
+  if (s.elt != 1 && s.elt != 2 && s.elt != 4 && s.elt != 8) return kBad;
+  if (s.tokens < 0 || s.tokens > kRowsMaxCount || s.pages < 1 || s.pageSize < 1) return kBad;
+  if (s.heads < 1 || s.heads > (1 << 16) || s.headSize < 1 || s.headSize > (1 << 16)) return kBad;
+  if ((long long)s.heads * s.headSize > kRowsMaxWidth) return kBad;
+  const long long top = 1LL << 58;   // bytes that a stride may span in all
+  if (s.slotStride < s.headSize || s.slotStride > top / s.elt / s.pageSize) return kBad;
+  if (s.headStride < s.headSize || s.headStride > top / s.elt / s.heads) return kBad;
+  if (s.pageStride < s.headSize || s.pageStride > top / s.elt / s.pages) return kBad;
+  return 0;
+}
+
+int check_rows_sort(const RowsShape& s, const void* expertOf, size_t sizeofIndex, const void* count,
+                    const void* offset, const void* rowOf, const void* slotOf) {
+  const bool any = (long long)s.tokens * s.choices > 0;
+  if (sizeofIndex != 4 && sizeofIndex != 8) return kBad;
+  if (!count || !offset || !slotOf || (any && (!expertOf || !rowOf))) return kBad;
+  const void* p[] = {expertOf, count, offset, rowOf, slotOf};
+  for (int i = 0; i < 5; i++)
+    for (int j = 0; j < i; j++)
+      if (p[i] && p[i] == p[j]) return kBad;
+  if (!aligned(expertOf, sizeofIndex)) return kBad;
+  for (const void* q : p)
+    if (!aligned(q, 4)) return kBad;
+  return 0;
+}
+
+int check_rows_move(const RowsShape& s, const RowsMoveArgs& a) {
+  const int elt = rows_element_bytes(s.type);
+  const long long top = (1LL << 58) / elt;
+  const long long slots = (long long)s.tokens * s.choices;
+  if (!a.row || a.token == a.row) return kBad;
+  if (slots && (!a.token || !a.rowOf)) return kBad;
+  if (a.needMap && (!a.count || !a.offset)) return kBad;
+  if (s.type == 0 && (a.weight || a.dweight || !a.rowsOut)) return kBad;
+  if ((a.dweight != nullptr) != (a.other != nullptr)) return kBad;
+  if (a.weight && a.weight == a.dweight) return kBad;
+  const void* out = a.rowsOut ? a.row : a.token;
+  if (a.other && a.other == out) return kBad;
+  if (!aligned(a.token, elt) || !aligned(a.row, elt) || !aligned(a.other, elt)) return kBad;
+  if (!aligned(a.rowOf, 4) || !aligned(a.count, 4) || !aligned(a.offset, 4) || !aligned(a.weight, 4) ||
+      !aligned(a.dweight, 4))
+    return kBad;
+  if (a.tokenStride < 0 || a.rowStride < 0 || a.otherStride < 0) return kBad;
+  if ((a.rowsOut ? a.rowStride : a.tokenStride) < s.width) return kBad;
+  if (a.tokenStride > top / (s.tokens + 1) || a.rowStride > top / s.capacity) return kBad;
+  // the other factor lies on the side that is written
+  if (a.other && a.otherStride > top / ((a.rowsOut ? s.capacity : s.tokens) + 1)) return kBad;
+  return 0;
+}
+
+int check_pages_build(const PagesShape& s, const void* held, const void* added, const void* freeList,
+                      const void* poolIn, const void* poolOut, const void* table, long long tableStride,
+                      const void* tokenOffset, const void* pageOffset, const void* slot) {
+  if (!held || !added || !table || !tokenOffset || (!slot && s.maxTokens)) return kBad;
+  const bool take = freeList != nullptr;
+  if (take != (poolIn != nullptr) || take != (poolOut != nullptr) || take != (pageOffset != nullptr)) return kBad;
+  if (tableStride < s.tableWidth || tableStride > (1LL << 56) / s.requests) return kBad;
+  const void* in[] = {held, added, freeList, poolIn};
+  const void* out[] = {table, tokenOffset, pageOffset, slot, poolOut};
+  for (const void* o : out) {
+    if (!o) continue;
+    for (const void* i : in)
+      if (i == o && !(o == poolOut && i == poolIn)) return kBad;
+  }
+  for (int i = 0; i < 5; i++)
+    for (int j = 0; j < i; j++)
+      if (out[i] && out[i] == out[j]) return kBad;
+  for (const void* p : in)
+    if (!aligned(p, 4)) return kBad;
+  for (const void* p : out)
+    if (!aligned(p, p == slot ? 8 : 4)) return kBad;
+  return 0;
+}
+
+int check_paged_move(const PagedShape& s, const void* k, const void* v, long long tokenStride,
+                     long long headStride, const void* slot, const void* kCache, const void* vCache,
+                     bool rowsOut) {
+  if (!k || !kCache || !slot || (v != nullptr) != (vCache != nullptr)) return kBad;
+  if (k == kCache || (v && (v == vCache || v == kCache || k == vCache))) return kBad;
+  if (v && (rowsOut ? k == v : kCache == vCache)) return kBad;
+  const void* p[] = {k, v, kCache, vCache};
+  for (const void* q : p)
+    if (!aligned(q, s.elt)) return kBad;
+  if (!aligned(slot, 8)) return kBad;
+  const long long low = rowsOut ? s.headSize : 0, top = (1LL << 58) / s.elt;
+  if (tokenStride < low || tokenStride > top / (s.tokens + 1)) return kBad;
+  if (headStride < low || headStride > top / s.heads) return kBad;
+  return 0;
+}
+
+int access_bytes(unsigned long long bits, int elt) {
+  int vb = 16;
+  while (vb > elt && bits % vb) vb >>= 1;
+  return vb;
+}
+
+}  // namespace cuttb

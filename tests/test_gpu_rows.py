@@ -1,0 +1,490 @@
+"""Rows sorted by expert, moved there and back, and the gradients, on the GPU against plain 64-bit
+arithmetic (cutt_rows_* of include/cutt_rows.h).
+
+Tolerances.  Every output is one rounding of a 32-bit result: half a step of the type relative to the
+value, plus what the 32-bit arithmetic loses - a product or a sum of n terms by at most n + 1 roundings
+of 2^-24 relative to the sum of the terms' magnitudes - plus half of the type's smallest step for values
+near zero.  Moves without weights are exact."""
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+HALF = {"f16": (2.0 ** -11, 2.0 ** -25), "bf16": (2.0 ** -8, 2.0 ** -134), "f32": (2.0 ** -24, 2.0 ** -150)}
+
+
+def _types(native):
+    import torch
+    return {"bytes": (native.CUTT_ROWS_BYTES, torch.uint8), "f16": (native.CUTT_ROWS_F16, torch.float16),
+            "bf16": (native.CUTT_ROWS_BF16, torch.bfloat16), "f32": (native.CUTT_ROWS_F32, torch.float32)}
+
+
+def plain_map(ids, first, experts, align, capacity):
+    """The map by its definition, slot by slot."""
+    ids = [int(x) - first for x in ids]
+    n = [0] * experts
+    for e in ids:
+        if 0 <= e < experts:
+            n[e] += 1
+    start, at = [], 0
+    for e in range(experts):
+        start.append(at)
+        at += -(-n[e] // align) * align
+    offset = [min(s, capacity) for s in start + [at]]
+    count = [min(start[e] + n[e], capacity) - min(start[e], capacity) for e in range(experts)]
+    row_of, slot_of, seen = [-1] * len(ids), [-1] * capacity, [0] * experts
+    for s, e in enumerate(ids):
+        if not 0 <= e < experts:
+            continue
+        r = start[e] + seen[e]
+        seen[e] += 1
+        if r < capacity:
+            row_of[s], slot_of[r] = r, s
+    return count, offset, row_of, slot_of
+
+
+class Run:
+    """Plan, map and device buffers of one routing."""
+
+    def __init__(self, native, ids, width, kind, experts, first=0, align=1, capacity=None, index=None):
+        import torch
+        self.torch, self.C = torch, native
+        t, k = ids.shape
+        self.t, self.k, self.h, self.kind = t, k, width, kind
+        self.code, self.dtype = _types(native)[kind]
+        self.plan = native.RowPlan(t, k, experts, width, self.code, first=first, align=align, capacity=capacity,
+                                   stream=torch.cuda.current_stream().cuda_stream)
+        self.r, self.e = self.plan.capacity, experts
+        self.ids = ids.to(index or torch.int32).cuda().contiguous()
+        i32 = dict(dtype=torch.int32, device="cuda")
+        self.count, self.offset = torch.full((experts,), -7, **i32), torch.full((experts + 1,), -7, **i32)
+        self.row_of, self.slot_of = torch.full((t, k), -7, **i32), torch.full((self.r,), -7, **i32)
+        self.want = plain_map(ids.reshape(-1).tolist(), first, experts, align, self.r)
+
+    def sort(self):
+        self.plan.sort(self.ids.data_ptr(), self.ids.element_size(), self.count.data_ptr(), self.offset.data_ptr(),
+                       self.row_of.data_ptr(), self.slot_of.data_ptr())
+
+    def check_map(self):
+        got = (self.count.tolist(), self.offset.tolist(), self.row_of.reshape(-1).tolist(), self.slot_of.tolist())
+        for name, g, w in zip(("count", "offset", "row_of", "slot_of"), got, self.want):
+            assert g == w, name
+
+    def maps(self):
+        return self.row_of.data_ptr(), self.count.data_ptr(), self.offset.data_ptr()
+
+    def rows(self, n, g, pad=0, shift=0):
+        """n rows; `pad` elements between rows, the first `shift` elements behind an aligned address."""
+        torch = self.torch
+        flat = torch.randn(shift + n * (self.h + pad) + 8, generator=g)
+        flat = (flat * 40).to(torch.uint8) if self.kind == "bytes" else flat.to(self.dtype)
+        return flat.cuda()[shift:shift + n * (self.h + pad)].view(n, self.h + pad)[:, :self.h]
+
+    def live(self):
+        row = self.torch.tensor(self.want[2]).view(self.t, self.k)
+        return row, row >= 0
+
+    def padding(self):
+        c, o = self.want[0], self.want[1]
+        return [r for e in range(self.e) for r in range(o[e] + c[e], o[e + 1])]
+
+
+def close(got, want, magnitude, terms, kind):
+    rel, least = HALF[kind]
+    got = got.double().cpu()
+    tol = rel * want.abs() * 1.001 + (terms + 1) * 2.0 ** -24 * magnitude * 1.001 + least
+    worst = ((got - want).abs() - tol).max().item() if got.numel() else -1
+    assert worst <= 0, worst
+
+
+def routing(t, k, e, seed, drop=0.0, first=0):
+    import torch
+    g = torch.Generator().manual_seed(seed)
+    k2 = min(k, e)
+    ids = torch.rand(t, e, generator=g).topk(k2, dim=1).indices if t else torch.zeros(0, k2, dtype=torch.int64)
+    if k > k2:                       # more choices than experts: experts come twice
+        ids = torch.cat([ids, torch.randint(0, e, (t, k - k2), generator=g)], 1)
+    ids = ids + first
+    if drop:
+        ids[torch.rand(t, k, generator=g) < drop] = first - 1
+    return ids
+
+
+MAPS = [(1, 1, 1, 1), (1, 8, 64, 1), (7, 3, 5, 4), (48, 6, 64, 1), (33, 8, 256, 16), (513, 4, 17, 128), (2000, 8, 384, 8),
+        (40000, 2, 300, 64), (257, 10, 4096, 1), (3, 5, 2, 7)]
+
+
+@pytest.mark.parametrize("t,k,e,align", MAPS)
+@pytest.mark.parametrize("drop", [0.0, 0.3])
+def test_map(native, t, k, e, align, drop):
+    import torch
+    r = Run(native, routing(t, k, e, t + e, drop, first=5), 8, "bf16", e, first=5, align=align,
+            index=torch.int64 if t % 2 else torch.int32)
+    r.sort()
+    r.check_map()
+
+
+def test_map_of_nothing_and_of_dropped_slots(native):
+    import torch
+    r = Run(native, torch.zeros(0, 4, dtype=torch.int64), 8, "bf16", 6, align=8, capacity=10)
+    r.sort()
+    r.check_map()
+    assert r.slot_of.tolist() == [-1] * 10
+    for value in (-1, 6, 2**31 - 1, -2**31, 2**62, -2**63):
+        r = Run(native, torch.full((70, 2), value), 8, "bf16", 6, align=8, index=torch.int64 if abs(value) > 2**31 else torch.int32)
+        r.sort()
+        r.check_map()
+        assert r.offset.tolist() == [0] * 7
+
+
+@pytest.mark.parametrize("t,capacity", [(100, 1), (100, 63), (100, 200), (5000, 4096), (5000, 9999)])
+def test_map_drops_what_does_not_fit(native, t, capacity):
+    r = Run(native, routing(t, 2, 9, 3), 8, "bf16", 9, align=16, capacity=capacity)
+    r.sort()
+    r.check_map()
+
+
+@pytest.mark.parametrize("t,k,e", [(30000, 2, 64), (131072, 1, 8), (20000, 8, 4096), (70001, 3, 129)])
+def test_map_one_expert_for_all_and_long_ones(native, t, k, e):
+    import torch
+    r = Run(native, torch.full((t, k), e - 1), 8, "bf16", e, align=128)
+    r.sort()
+    r.check_map()
+    r = Run(native, routing(t, k, e, 9, 0.1), 8, "bf16", e, align=128)
+    r.sort()
+    r.check_map()
+
+
+SHAPES = [  # tokens, choices, experts, width, align, pad, shift, drop
+    (1, 8, 16, 512, 1, 0, 0, 0.0), (5, 1, 3, 1, 1, 0, 0, 0.0), (48, 6, 64, 2048, 1, 8, 0, 0.0), (33, 3, 7, 1111, 1, 0, 0, 0.2),
+    (64, 4, 16, 264, 16, 0, 1, 0.2), (17, 10, 12, 136, 128, 24, 0, 0.3), (300, 2, 8, 40, 8, 3, 0, 0.9), (6000, 5, 24, 72, 8, 0, 0, 0.1),
+    (5000, 9, 24, 33, 1, 0, 0, 0.0), (9, 3, 2, 4100, 64, 0, 0, 0.0)]
+
+
+@pytest.mark.parametrize("kind", ["bytes", "f16", "bf16", "f32"])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_dispatch(native, kind, shape):
+    import torch
+    t, k, e, h, align, pad, shift, drop = shape
+    r = Run(native, routing(t, k, e, 11, drop), h, kind, e, align=align)
+    r.sort()
+    g = torch.Generator().manual_seed(1)
+    x = r.rows(t, g, pad, shift)
+    row, ok = r.live()
+    for weighted in ([False] if kind == "bytes" else [False, True]):
+        w = torch.randn(t, k, generator=g) if weighted else None
+        y = torch.full((r.r, h + pad), 77, dtype=r.dtype, device="cuda")
+        r.plan.dispatch(x.data_ptr(), *r.maps(), y.data_ptr(), weight=w.cuda().data_ptr() if weighted else 0,
+                        x_stride=x.stride(0), y_stride=y.stride(0))
+        assert (y[:, h:] == 77).all()                     # between the rows nothing is written
+        got, xs = y[:, :h].cpu(), x.cpu()
+        used = r.want[1][-1]
+        assert (got[used:] == 77).all()                   # rows behind the last segment are left alone
+        assert (got[r.padding()] == 0).all()
+        src = xs[:, None, :].expand(t, k, h)[ok]
+        if weighted:
+            want = src.double() * w.double()[ok][:, None]
+            close(got[row[ok].long()], want, want.abs(), 1, kind)
+        else:
+            assert torch.equal(got[row[ok].long()], src)
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_combine(native, kind, shape):
+    import torch
+    t, k, e, h, align, pad, shift, drop = shape
+    r = Run(native, routing(t, k, e, 12, drop), h, kind, e, align=align)
+    r.sort()
+    g = torch.Generator().manual_seed(2)
+    y = r.rows(r.r, g, pad, shift)
+    y[r.padding()] = float("nan")                         # rows that no slot owns are not read
+    y[r.want[1][-1]:] = float("nan")
+    row, ok = r.live()
+    ys = y.double().cpu()
+    parts = torch.where(ok[:, :, None], ys[row.clamp_min(0).long()], 0.0)
+    for weighted in (False, True):
+        w = torch.randn(t, k, generator=g) if weighted else torch.ones(t, k)
+        w[~ok] = float("nan")                             # nor are their weights
+        out = torch.full((t, h + pad), 77, dtype=r.dtype, device="cuda")
+        r.plan.combine(y.data_ptr(), r.row_of.data_ptr(), out.data_ptr(), weight=w.cuda().data_ptr() if weighted else 0,
+                       y_stride=y.stride(0), out_stride=out.stride(0))
+        assert (out[:, h:] == 77).all()
+        terms = torch.where(ok[:, :, None], parts * w.double()[:, :, None], 0.0)
+        close(out[:, :h], terms.sum(1), terms.abs().sum(1), k, kind)
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_gradients(native, kind, shape):
+    import torch
+    t, k, e, h, align, pad, shift, drop = shape
+    r = Run(native, routing(t, k, e, 13, drop), h, kind, e, align=align)
+    r.sort()
+    g = torch.Generator().manual_seed(3)
+    token, rows = r.rows(t, g, pad, shift), r.rows(r.r, g, pad, shift)
+    rows[r.padding()] = float("nan")
+    row, ok = r.live()
+    ts, rs = token.double().cpu(), rows.double().cpu()
+    parts = torch.where(ok[:, :, None], rs[row.clamp_min(0).long()], 0.0)
+    products = parts * ts[:, None, :]
+    for weighted in (False, True):
+        w = torch.randn(t, k, generator=g)
+        wd = w.double() if weighted else torch.ones(t, k, dtype=torch.float64)
+        wp = w.cuda()
+        for want_dw in (False, True):
+            dw = torch.full((t, k), 77.0, device="cuda")
+            # the gradient of combine: rows written, the token side read
+            dy = torch.full((r.r, h + pad), 77, dtype=r.dtype, device="cuda")
+            r.plan.combine_grad(token.data_ptr(), *r.maps(), dy.data_ptr(), weight=wp.data_ptr() if weighted else 0,
+                                y=rows.data_ptr() if want_dw else 0, dweight=dw.data_ptr() if want_dw else 0,
+                                dout_stride=token.stride(0), y_stride=rows.stride(0), dy_stride=dy.stride(0))
+            got = dy[:, :h].cpu()
+            assert (got[r.want[1][-1]:] == 77).all() and (dy[:, h:] == 77).all() and (got[r.padding()] == 0).all()
+            want = (ts[:, None, :] * wd[:, :, None])[ok]
+            close(got[row[ok].long()], want, want.abs() if weighted else want * 0, 1, kind)
+            if want_dw:
+                close(dw, products.sum(2), products.abs().sum(2), h, "f32")
+                assert (dw.cpu()[~ok] == 0).all()
+            # the gradient of dispatch: the token side written
+            dx = torch.full((t, h + pad), 77, dtype=r.dtype, device="cuda")
+            dw.fill_(77.0)
+            r.plan.dispatch_grad(rows.data_ptr(), r.row_of.data_ptr(), dx.data_ptr(), weight=wp.data_ptr() if weighted else 0,
+                                 x=token.data_ptr() if want_dw else 0, dweight=dw.data_ptr() if want_dw else 0,
+                                 dy_stride=rows.stride(0), x_stride=token.stride(0), dx_stride=dx.stride(0))
+            terms = parts * wd[:, :, None]
+            close(dx[:, :h], terms.sum(1), terms.abs().sum(1), k, kind)
+            assert (dx[:, h:] == 77).all()
+            if want_dw:
+                close(dw, products.sum(2), products.abs().sum(2), h, "f32")
+                assert (dw.cpu()[~ok] == 0).all()
+            else:
+                assert (dw == 77).all()
+
+
+def test_broadcast_inputs(native):
+    """Inputs of row stride 0: an expanded gradient, one row for all."""
+    import torch
+    r = Run(native, routing(50, 3, 6, 1), 64, "bf16", 6, align=4)
+    r.sort()
+    one = torch.randn(64).bfloat16().cuda()
+    y = torch.zeros(r.r, 64, dtype=torch.bfloat16, device="cuda")
+    r.plan.combine_grad(one.data_ptr(), *r.maps(), y.data_ptr(), dout_stride=0)
+    row, ok = r.live()
+    assert torch.equal(y[row[ok].long().cuda()], one.expand(int(ok.sum()), 64))
+    out = torch.zeros(50, 64, dtype=torch.bfloat16, device="cuda")
+    r.plan.combine(one.data_ptr(), r.row_of.data_ptr(), out.data_ptr(), y_stride=0)
+    close(out, 3 * one.double().cpu().expand(50, 64), 3 * one.double().cpu().abs().expand(50, 64), 3, "bf16")
+
+
+def test_not_a_number_stays_in_its_row(native):
+    import torch
+    r = Run(native, routing(40, 4, 8, 2), 256, "f32", 8)
+    r.sort()
+    y = torch.randn(r.r, 256, device="cuda")
+    row, _ = r.live()
+    y[row[7, 2]] = float("nan")
+    y[row[9, 0], 3] = float("inf")
+    out = torch.zeros(40, 256, device="cuda")
+    r.plan.combine(y.data_ptr(), r.row_of.data_ptr(), out.data_ptr())
+    bad = ~torch.isfinite(out)
+    assert bad[7].all() and bad[9, 3] and bad.sum().item() == 257
+
+
+def test_maps_out_of_range_are_taken_as_dropped(native):
+    """A damaged map: entries beyond the capacity move nothing."""
+    import torch
+    r = Run(native, routing(20, 2, 4, 4), 32, "f32", 4)
+    r.sort()
+    r.row_of.view(-1)[5] = r.r
+    r.row_of.view(-1)[6] = 2**31 - 1
+    r.row_of.view(-1)[7] = -2**31
+    x = torch.randn(20, 32, device="cuda")
+    y = torch.full((r.r, 32), 77.0, device="cuda")
+    r.plan.dispatch(x.data_ptr(), *r.maps(), y.data_ptr())
+    want = torch.full((r.r, 32), 77.0, device="cuda")
+    for s, p in enumerate(r.row_of.view(-1).tolist()):
+        if 0 <= p < r.r:
+            want[p] = x[s // 2]
+    assert torch.equal(y, want)
+    out = torch.zeros(20, 32, device="cuda")
+    r.plan.combine(y.data_ptr(), r.row_of.data_ptr(), out.data_ptr())
+    assert torch.equal(out[0], 2 * x[0]) and torch.equal(out[3], 0 * x[3])
+
+
+def _layer(native, t, k, e, h, kind, align, stream=0):
+    """A layer of experts as a user writes it: forward and backward through the row operators, the experts'
+    products by segments of the sorted rows."""
+    import torch
+
+    class Layer:
+        plan = native.RowPlan(t, k, e, h, _types(native)[kind][0], align=align, stream=stream)
+        dtype = _types(native)[kind][1]
+
+        def __init__(self):
+            r, i32 = self.plan.capacity, dict(dtype=torch.int32, device="cuda")
+            self.count, self.offset = torch.zeros(e, **i32), torch.zeros(e + 1, **i32)
+            self.row_of, self.slot_of = torch.zeros(t, k, **i32), torch.zeros(r, **i32)
+            new = lambda *s: torch.zeros(*s, dtype=self.dtype, device="cuda")
+            self.rows, self.y, self.dy, self.drows = new(r, h), new(r, h), new(r, h), new(r, h)
+            self.out, self.dx, self.dw = new(t, h), new(t, h), torch.zeros(t, k, device="cuda")
+
+        def forward(self, x, ids, w, scale):
+            p = self.plan
+            p.sort(ids.data_ptr(), ids.element_size(), self.count.data_ptr(), self.offset.data_ptr(), self.row_of.data_ptr(),
+                   self.slot_of.data_ptr())
+            p.dispatch(x.data_ptr(), self.row_of.data_ptr(), self.count.data_ptr(), self.offset.data_ptr(), self.rows.data_ptr())
+            self.expert = (torch.searchsorted(self.offset[1:].contiguous(), torch.arange(p.capacity, device="cuda", dtype=torch.int32),
+                                              right=True)).clamp_max(e - 1)
+            self.y.copy_(self.rows * scale[self.expert])
+            p.combine(self.y.data_ptr(), self.row_of.data_ptr(), self.out.data_ptr(), weight=w.data_ptr())
+            return self.out
+
+        def backward(self, dout, w, scale):
+            p = self.plan
+            p.combine_grad(dout.data_ptr(), self.row_of.data_ptr(), self.count.data_ptr(), self.offset.data_ptr(), self.dy.data_ptr(),
+                           weight=w.data_ptr(), y=self.y.data_ptr(), dweight=self.dw.data_ptr())
+            self.drows.copy_(self.dy * scale[self.expert])
+            self.dscale = torch.zeros_like(scale).index_add_(0, self.expert, self.dy * self.rows)
+            p.dispatch_grad(self.drows.data_ptr(), self.row_of.data_ptr(), self.dx.data_ptr())
+            return self.dx, self.dw, self.dscale
+    return Layer()
+
+
+def test_layer_forward_and_backward(native):
+    """All operators together: outputs and gradients against autograd in 64 bits and against differences."""
+    import torch
+    t, k, e, h = 29, 3, 5, 48
+    g = torch.Generator().manual_seed(8)
+    ids = routing(t, k, e, 21, 0.1)
+    x, w, scale = torch.randn(t, h, generator=g), torch.randn(t, k, generator=g), torch.randn(e, h, generator=g)
+    dout = torch.randn(t, h, generator=g)
+    layer = _layer(native, t, k, e, h, "f32", 8)
+    ws, sc = w.cuda(), scale.cuda()
+    out = layer.forward(x.cuda(), ids.int().cuda(), ws, sc).cpu()
+    dx, dw, dscale = [v.cpu() for v in layer.backward(dout.cuda(), ws, sc)]
+
+    def plain(x, w, scale):
+        ok = (ids >= 0).double()[:, :, None]
+        return (x[:, None, :] * scale[ids.clamp_min(0)] * w[:, :, None] * ok).sum(1)
+
+    xd, wd, sd = [v.double().requires_grad_() for v in (x, w, scale)]
+    want = plain(xd, wd, sd)
+    want.backward(dout.double())
+    # three products in a row and a sum of k (dx, out) or h (dw) or t * k (dscale) terms
+    big = 16.0 * 16 * 16
+    for got, ref, n in ((out, want.detach(), k), (dx, xd.grad, k), (dw, wd.grad, h), (dscale, sd.grad, t * k)):
+        assert (got.double() - ref).abs().max().item() <= (n + 4) * n * 2.0 ** -24 * big
+    # differences of the operators' own forward pass: d/dx in a direction; the layer is linear in x, so the
+    # difference quotient is exact up to rounding (2^-24 of the outputs' size, over the step)
+    step, direction = 2.0 ** -4, torch.randn(t, h, generator=g)
+    loss = lambda xs: (layer.forward(xs.cuda(), ids.int().cuda(), ws, sc).cpu().double() * dout.double()).sum().item()
+    slope = (loss(x + step * direction) - loss(x - step * direction)) / (2 * step)
+    assert abs(slope - (dx.double() * direction.double()).sum().item()) <= t * h * (k + 4) * 2.0 ** -24 * big / step / 16
+    loss_w = lambda ws_: (layer.forward(x.cuda(), ids.int().cuda(), ws_.cuda(), sc).cpu().double() * dout.double()).sum().item()
+    direction = torch.randn(t, k, generator=g)
+    slope = (loss_w(w + step * direction) - loss_w(w - step * direction)) / (2 * step)
+    assert abs(slope - (dw.double() * direction.double()).sum().item()) <= t * h * (k + 4) * 2.0 ** -24 * big / step / 16
+
+
+def test_layer_captured_and_replayed_with_new_routing(native):
+    """A whole step in a CUDA graph on the plan's stream; replays read the routing that is in the buffers then,
+    while an eager layer of the same inputs lives.  Results equal the eager ones bit for bit."""
+    import torch
+    t, k, e, h = 600, 4, 32, 256
+    side = torch.cuda.Stream()
+    captured, eager = _layer(native, t, k, e, h, "bf16", 16, side.cuda_stream), _layer(native, t, k, e, h, "bf16", 16)
+    g = torch.Generator().manual_seed(4)
+    ids = routing(t, k, e, 1).int().cuda()
+    x, dout = torch.randn(t, h, generator=g).bfloat16().cuda(), torch.randn(t, h, generator=g).bfloat16().cuda()
+    w, scale = torch.rand(t, k, generator=g).cuda(), torch.randn(e, h, generator=g).bfloat16().cuda()
+    eager.forward(x, ids, w, scale)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        captured.forward(x, ids, w, scale)
+        captured.backward(dout, w, scale)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        captured.forward(x, ids, w, scale)
+        captured.backward(dout, w, scale)
+    for seed in (2, 3):
+        ids.copy_(routing(t, k, e, seed, 0.2 * (seed - 2)).int().cuda())
+        x.copy_(torch.randn(t, h, generator=g).bfloat16().cuda())
+        for layer in (captured, eager):
+            layer.rows.zero_()
+            layer.dy.zero_()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        eager.forward(x, ids, w, scale)
+        eager.backward(dout, w, scale)
+        torch.cuda.synchronize()
+        for name in ("row_of", "slot_of", "rows", "out", "dy", "dx", "dw"):
+            assert torch.equal(getattr(captured, name), getattr(eager, name)), name
+
+
+def test_two_plans_on_two_streams_at_once(native):
+    import torch
+    sets = []
+    for i in range(2):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            sets.append((s, Run(native, routing(3000, 4, 40, 30 + i), 512, "bf16", 40, align=8)))
+    torch.cuda.synchronize()
+    xs = [torch.randn(3000, 512, device="cuda").bfloat16() for _ in sets]
+    ys = [torch.zeros(r.r, 512, dtype=torch.bfloat16, device="cuda") for _, r in sets]
+    outs = [torch.zeros(3000, 512, dtype=torch.bfloat16, device="cuda") for _ in sets]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for (_, r), x, y, out in zip(sets, xs, ys, outs):
+            r.sort()
+            r.plan.dispatch(x.data_ptr(), *r.maps(), y.data_ptr())
+            r.plan.combine(y.data_ptr(), r.row_of.data_ptr(), out.data_ptr())
+    torch.cuda.synchronize()
+    for (_, r), x, out in zip(sets, xs, outs):
+        r.check_map()
+        assert torch.equal(out, (4 * x.float()).bfloat16())     # four copies of a row: exact
+
+
+def test_handles_and_devices(native):
+    import torch
+    n0 = native.launch_count()
+    r = Run(native, routing(4, 2, 4, 0), 16, "bf16", 4)
+    h = r.plan.handle
+    assert '"rows"' in r.plan.describe()
+    assert native.cuttExecute(h, 16, 32) == native.CUTT_INVALID_PLAN
+    L = native.lib()
+    assert L.cutt_pages_store(h, 16, 0, 8, 8, 32, 48, 0) == native.CUTT_INVALID_PLAN       # a handle of another kind
+    x = torch.zeros(4, 16, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(native.CuttError) as bad:
+        r.plan.dispatch(x.data_ptr(), *r.maps(), x.data_ptr())
+    assert bad.value.code == native.CUTT_INVALID_PARAMETER
+    assert native.launch_count() == n0
+    r.sort()
+    assert native.launch_count() > n0
+    r.plan.destroy()
+    assert native.cuttDestroy(h) == native.CUTT_INVALID_PLAN
+    with pytest.raises(native.CuttError):
+        r.plan.describe()
+    with pytest.raises(native.CuttError):
+        r.sort()
+
+
+def test_row_offsets_beyond_32_bits(native):
+    """Rows whose byte offsets pass 2^32 (and whose element offsets pass 2^31)."""
+    import torch
+    t, k, e, h = 40, 2, 3, 1 << 20
+    stride = (1 << 26) + 8
+    r = Run(native, routing(t, k, e, 5), 512, "bf16", e)
+    r.sort()
+    x = torch.randn(t, 512, device="cuda").bfloat16()
+    y = torch.zeros(stride * (r.r - 1) + 512, dtype=torch.bfloat16, device="cuda")
+    assert y.numel() > 2**32
+    r.plan.dispatch(x.data_ptr(), *r.maps(), y.data_ptr(), y_stride=stride)
+    rows = torch.as_strided(y, (r.r, 512), (stride, 1))
+    row, ok = r.live()
+    assert torch.equal(rows[row.view(-1).long().cuda()], x[:, None].expand(t, k, 512).reshape(-1, 512))
+    out = torch.zeros_like(x)
+    r.plan.combine(y.data_ptr(), r.row_of.data_ptr(), out.data_ptr(), y_stride=stride)
+    assert torch.equal(out, (2 * x.float()).bfloat16())
