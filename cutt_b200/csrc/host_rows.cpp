@@ -1,5 +1,5 @@
 // Test-only: the argument checks and the index arithmetic of the row operators on the host.
-#include <vector>
+#include <string.h>
 
 #include "rows_plan.h"
 
@@ -101,6 +101,32 @@ long long cutt_hostcheck_pages_run(int requests, int pageSize, int tableWidth, i
 long long cutt_hostcheck_cache_offset(int pages, int pageSize, long long pageStride, long long slotStride, long long slot) {
   const PagedShape s{1, 1, 1, 1, pages, pageSize, pageStride, slotStride, 1};
   return cache_offset(s, slot, make_fastdiv(pageSize));
+}
+
+// cutt_pages_store / cutt_pages_load of one tensor on host arrays, access by access as the blocks do
+// it.  Returns the accesses outside the arrays (rowBytes, cacheBytes) or off their alignment, which
+// are skipped.
+long long cutt_hostcheck_paged_run(const int* shape, const long long* strides, long long tokenStride, long long headStride,
+                                   const long long* slot, unsigned char* rows, long long rowBytes, unsigned char* cache,
+                                   long long cacheBytes, int store) {
+  const PagedShape s{shape[0], shape[1], shape[2], shape[3], shape[4], shape[5], strides[0], strides[1], strides[2]};
+  const PagedItems p = paged_items(s, tokenStride * s.elt, headStride * s.elt, (uintptr_t)rows | (uintptr_t)cache);
+  long long bad = 0;
+  for (int q0 = 0; q0 < s.tokens; q0 += p.perBlock) {
+    const int nq = p.perBlock < s.tokens - q0 ? p.perBlock : s.tokens - q0;
+    for (uint32_t i = 0; i < (uint32_t)nq * p.vecs; i++) {
+      long long c, r;
+      if (!paged_item(p, slot, q0, i, c, r)) continue;
+      if (c < 0 || r < 0 || c + p.access > cacheBytes || r + p.access > rowBytes || (uintptr_t)(cache + c) % p.access ||
+          (uintptr_t)(rows + r) % p.access) {
+        bad++;
+        continue;
+      }
+      if (store) memcpy(cache + c, rows + r, p.access);
+      else memcpy(rows + r, cache + c, p.access);
+    }
+  }
+  return bad;
 }
 
 int cutt_hostcheck_local_expert(long long e, int first, int experts) { return local_expert(e, first, experts); }

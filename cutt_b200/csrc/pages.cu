@@ -1,5 +1,6 @@
 // Block tables and slot maps from request lengths (cutt_pages_build), and rows stored into and
 // loaded from pages (cutt_pages_store, cutt_pages_load).
+#include <cooperative_groups.h>
 #include <stdint.h>
 
 #include "kernels.h"
@@ -11,67 +12,110 @@ namespace {
 
 constexpr unsigned kFull = 0xffffffffu;
 
-__device__ __forceinline__ long long block_scan64(long long v, long long* s, long long& total) {
+// Sum of two counts that stops at 2^31 - 1.  Associative, so a scan with it is the saturated scan.
+__device__ __forceinline__ unsigned add_up_to_int(unsigned a, unsigned b) { return min(a + b, 0x7fffffffu); }
+
+// Exclusive prefix sums of (tokens, pages) over the block: tokens saturate, pages cannot overflow
+// (a table has fewer than 2^30 entries).
+__device__ __forceinline__ uint2 block_scan2(uint2 v, uint2* s, uint2& total) {
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, nw = blockDim.x >> 5;
-  long long x = v;
+  uint2 x = v;
+#pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
-    const long long y = __shfl_up_sync(kFull, x, d);
-    if (lane >= d) x += y;
+    const unsigned t = __shfl_up_sync(kFull, x.x, d), p = __shfl_up_sync(kFull, x.y, d);
+    if (lane >= d) {
+      x.x = add_up_to_int(x.x, t);
+      x.y += p;
+    }
   }
+  uint2 before;                  // exclusive within the warp
+  before.x = __shfl_up_sync(kFull, x.x, 1);
+  before.y = __shfl_up_sync(kFull, x.y, 1);
+  if (lane == 0) before = make_uint2(0, 0);
   if (lane == 31) s[w] = x;
   __syncthreads();
-  if (w == 0) {
-    long long t = lane < nw ? s[lane] : 0;
-    for (int d = 1; d < 32; d <<= 1) {
-      const long long y = __shfl_up_sync(kFull, t, d);
-      if (lane >= d) t += y;
+  uint2 y = lane < nw ? s[lane] : make_uint2(0, 0);      // every warp scans the warps' sums
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const unsigned t = __shfl_up_sync(kFull, y.x, d), p = __shfl_up_sync(kFull, y.y, d);
+    if (lane >= d) {
+      y.x = add_up_to_int(y.x, t);
+      y.y += p;
     }
-    if (lane < nw) s[lane] = t;
+  }
+  total.x = __shfl_sync(kFull, y.x, nw - 1);
+  total.y = __shfl_sync(kFull, y.y, nw - 1);
+  const unsigned bx = __shfl_sync(kFull, y.x, w > 0 ? w - 1 : 0), by = __shfl_sync(kFull, y.y, w > 0 ? w - 1 : 0);
+  if (w > 0) {
+    before.x = add_up_to_int(before.x, bx);
+    before.y += by;
   }
   __syncthreads();
-  const long long before = w ? s[w - 1] : 0;
-  total = s[nw - 1];
-  __syncthreads();
-  return before + x - v;
+  return before;
 }
 
-// Prefix sums of the new tokens and of the pages they take (a block).
-__device__ void scan_requests(const PagesBuild& p, const int* poolIn, int* poolOut, int* tokenOffset, int* pageOffset) {
-  __shared__ long long s[33];
-  long long tokens = 0, pages = 0;
-  int limit = 0, first = 0;
+// Prefix sums of the new tokens and of the pages they take, by one block: to shared memory (toks,
+// pags) where those are given, to tokenOffset and pageOffset where `writes` is set.
+struct Pool {
+  int first, limit, entries;      // next free entry and number of entries of the free list, clamped; as given
+};
+__device__ __forceinline__ Pool read_pool(const PagesBuild& p, const int* poolIn) {
+  Pool r = {0, 0, 0};
   if (p.freeList) {
-    first = clamp_pool(poolIn[0]);
-    limit = clamp_pool(poolIn[1]);
-    pages = first;
+    r.first = clamp_pool(poolIn[0]);
+    r.entries = poolIn[1];
+    r.limit = clamp_pool(r.entries);
   }
+  return r;
+}
+__device__ __forceinline__ uint2 scan_requests(const PagesBuild& p, const Pool& pool, int* tokenOffset, int* pageOffset, bool writes,
+                                               int* toks, int* pags) {
+  __shared__ uint2 s[32];
+  unsigned tokens = 0, pages = pool.first;
   for (int b0 = 0; b0 < p.s.requests; b0 += blockDim.x) {
     const int b = b0 + threadIdx.x;
-    const int n = b < p.s.requests ? max(0, p.added[b]) : 0;
-    long long total;
-    const long long at = tokens + block_scan64(n, s, total);
-    tokens += total;
-    if (b < p.s.requests) tokenOffset[b] = saturate(at);
-    if (p.freeList) {
-      const int g = b < p.s.requests ? pages_taken(p.held[b], n, p.s.pageSize, p.s.tableWidth) : 0;
-      const long long f = pages + block_scan64(g, s, total);
-      pages += total;
-      if (b < p.s.requests) pageOffset[b] = (int)f;   // below 2^31: the table's entries and the pool are at most 2^30
+    const bool in = b < p.s.requests;
+    const int n = in ? max(0, p.added[b]) : 0;
+    const int g = in && p.freeList ? pages_taken(p.held[b], n, p.s.pageSize, p.s.tableWidth) : 0;
+    uint2 total;
+    const uint2 at = block_scan2(make_uint2(n, g), s, total);
+    if (in) {
+      const int t = (int)add_up_to_int(tokens, at.x), f = (int)(pages + at.y);
+      if (writes) {
+        tokenOffset[b] = t;
+        if (p.freeList) pageOffset[b] = f;
+      }
+      if (toks) {
+        toks[b] = t;
+        pags[b] = f;
+      }
     }
+    tokens = add_up_to_int(tokens, total.x);
+    pages += total.y;
   }
   if (threadIdx.x == 0) {
-    tokenOffset[p.s.requests] = saturate(tokens);
-    if (p.freeList) {
-      pageOffset[p.s.requests] = (int)pages;
-      poolOut[0] = min((int)pages, max(first, limit));
-      poolOut[1] = poolIn[1];
+    if (writes) {
+      tokenOffset[p.s.requests] = (int)tokens;
+      if (p.freeList) pageOffset[p.s.requests] = (int)pages;
+    }
+    if (toks) {
+      toks[p.s.requests] = (int)tokens;
+      pags[p.s.requests] = (int)pages;
     }
   }
+  return make_uint2(tokens, pages);
+}
+__device__ __forceinline__ void write_pool(const PagesBuild& p, const Pool& pool, unsigned pages, int* poolOut) {
+  if (!p.freeList || threadIdx.x != 0) return;
+  poolOut[0] = min((int)pages, max(pool.first, pool.limit));
+  poolOut[1] = pool.entries;
 }
 
-__device__ void expand_requests(const PagesBuild& p, int limit, int block, int blocks) {
+// Slots and new table entries, a part of them for each of `blocks` blocks.
+__device__ __forceinline__ void expand_requests(const PagesBuild& p, int limit, int block, int blocks) {
   const int stride = blocks * blockDim.x, at = block * blockDim.x + threadIdx.x;
   const int tokens = p.tokenOffset[p.s.requests];
+#pragma unroll 2
   for (int q = at; q < p.s.maxTokens; q += stride) {
     long long slot = -1;
     if (q < tokens) slot = slot_of_token(p, last_at_or_before(p.tokenOffset, p.s.requests + 1, q), q, limit);
@@ -83,11 +127,45 @@ __device__ void expand_requests(const PagesBuild& p, int limit, int block, int b
     take_page(p, last_at_or_before(p.pageOffset, p.s.requests + 1, f), f, limit);
 }
 
+// One kernel.  Every block makes all prefix sums for itself, in shared memory: a few kilobytes of
+// lengths, and no exchange.  Table entries that are read (pages of held tokens) and written (new ones)
+// differ, and slots of new pages come from the free list, so blocks wait for nothing - unless the
+// pool is updated in place (`inPlace`): then the blocks are one cluster, and the pool is written
+// after all of them have read it.
+constexpr int kSharedRequests = 4096;
+constexpr int kMostBlocks = 16;
+
 __global__ void __launch_bounds__(1024)
-pages_one_block(const __grid_constant__ PagesBuild p, const int* poolIn, int* poolOut, int* tokenOffset, int* pageOffset) {
-  scan_requests(p, poolIn, poolOut, tokenOffset, pageOffset);
-  __syncthreads();
-  expand_requests(p, p.freeList ? clamp_pool(poolOut[1]) : 0, 0, 1);
+pages_build(const __grid_constant__ PagesBuild p, const int* poolIn, int* poolOut, int* tokenOffset, int* pageOffset, bool inPlace) {
+  extern __shared__ int smem[];
+  int* toks = smem;
+  int* pags = smem + p.s.requests + 1;
+  const Pool pool = read_pool(p, poolIn);
+  const uint2 sums = scan_requests(p, pool, tokenOffset, pageOffset, blockIdx.x == 0, toks, pags);
+  if (inPlace) cooperative_groups::this_cluster().sync();
+  else __syncthreads();
+  if (blockIdx.x == 0) write_pool(p, pool, sums.y, poolOut);
+  PagesBuild q = p;
+  q.tokenOffset = toks;
+  q.pageOffset = pags;
+  expand_requests(q, pool.limit, blockIdx.x, gridDim.x);
+}
+
+// Two kernels: prefix sums by one block, then the rest by many.
+__global__ void __launch_bounds__(1024)
+pages_scan(const __grid_constant__ PagesBuild p, const int* poolIn, int* poolOut, int* tokenOffset, int* pageOffset) {
+  cudaTriggerProgrammaticLaunchCompletion();
+  const Pool pool = read_pool(p, poolIn);
+  const uint2 sums = scan_requests(p, pool, tokenOffset, pageOffset, true, nullptr, nullptr);
+  __syncthreads();          // every thread has read the pool, which may be updated in place
+  write_pool(p, pool, sums.y, poolOut);
+}
+
+constexpr int kExpandThreads = 256;
+
+__global__ void __launch_bounds__(kExpandThreads) pages_expand(const __grid_constant__ PagesBuild p) {
+  cudaGridDependencySynchronize();
+  expand_requests(p, p.freeList ? clamp_pool(p.pool[1]) : 0, blockIdx.x, gridDim.x);
 }
 
 template <int VB> struct Raw;
@@ -98,74 +176,112 @@ template <> struct Raw<2> { typedef uint16_t T; };
 template <> struct Raw<1> { typedef uint8_t T; };
 
 struct PagedLaunch {
-  PagedShape s;
+  PagedItems p;
   PagedMove m;
-  FastDiv divPage, divRow, divHead;   // by pageSize, by accesses of a token, by accesses of a head
-  int perBlock;                       // tokens of a block
-  int vecs;                           // accesses of a token
 };
 
-constexpr int kPagedThreads = 256;
-
-// grid.x: groups of perBlock tokens, grid.y: tensors.
+// grid.x: groups of perBlock tokens, grid.y: tensors.  A thread's loads are all issued before its first
+// store: with 1, 2, 4 and 8 of them 131072 K and V rows of 2 KB took 222, 197, 193 and 217 us.  Loads
+// and stores marked as not to be used again (ld.cs, st.cs) made that 180, and 8192 rows stored before
+// 131072 are loaded 192 instead of 207: the marked lines make room for one another.
 template <int VB>
-__global__ void __launch_bounds__(kPagedThreads) paged_kernel(const __grid_constant__ PagedLaunch p) {
+__global__ void __launch_bounds__(kPagedThreads) paged_kernel(const __grid_constant__ PagedLaunch l) {
   typedef typename Raw<VB>::T R;
-  const int q0 = blockIdx.x * p.perBlock;
-  const int nq = min(p.perBlock, p.s.tokens - q0);
-  const unsigned char* src = p.m.src[blockIdx.y];
-  unsigned char* dst = p.m.dst[blockIdx.y];
-  const uint32_t items = (uint32_t)nq * p.vecs;
-  for (uint32_t i = threadIdx.x; i < items; i += kPagedThreads) {
-    const uint32_t q = fdiv(i, p.divRow), r = i - q * p.vecs;
-    const uint32_t h = fdiv(r, p.divHead), v = r - h * p.divHead.d;
-    const long long at = cache_offset(p.s, p.m.slot[q0 + q], p.divPage);
-    if (at < 0) continue;
-    const long long c = (at + h * p.s.headStride) * p.s.elt + (long long)v * VB;
-    const long long x = (long long)(q0 + q) * p.m.tokenStride + h * p.m.headStride + (long long)v * VB;
-    if (p.m.store) *(R*)(dst + c) = *(const R*)(src + x);
-    else *(R*)(dst + x) = *(const R*)(src + c);
+  const int q0 = blockIdx.x * l.p.perBlock;
+  const unsigned char* src = l.m.src[blockIdx.y];
+  unsigned char* dst = l.m.dst[blockIdx.y];
+  const uint32_t items = (uint32_t)min(l.p.perBlock, l.p.s.tokens - q0) * l.p.vecs;
+  for (uint32_t i0 = threadIdx.x; i0 < items; i0 += kPagedThreads * kPagedItems) {
+    R value[kPagedItems];
+    R* to[kPagedItems];
+#pragma unroll
+    for (int k = 0; k < kPagedItems; k++) {
+      const uint32_t i = i0 + k * kPagedThreads;
+      long long cache, row;
+      to[k] = nullptr;
+      if (i >= items || !paged_item(l.p, l.m.slot, q0, i, cache, row)) continue;
+      value[k] = __ldcs((const R*)(src + (l.m.store ? row : cache)));
+      to[k] = (R*)(dst + (l.m.store ? cache : row));
+    }
+#pragma unroll
+    for (int k = 0; k < kPagedItems; k++)
+      if (to[k]) __stcs(to[k], value[k]);
   }
 }
 
 template <int VB>
-cudaError_t paged_vec(PagedLaunch& p, cudaStream_t stream) {
-  const int perHead = p.s.headSize * p.s.elt / VB;
-  p.vecs = perHead * p.s.heads;
-  p.divHead = make_fastdiv(perHead);
-  p.divRow = make_fastdiv(p.vecs);
-  p.perBlock = p.vecs >= kPagedThreads ? 1 : kPagedThreads / p.vecs;
-  const dim3 grid((unsigned)((p.s.tokens + p.perBlock - 1) / p.perBlock), p.m.tensors, 1);
-  paged_kernel<VB><<<grid, kPagedThreads, 0, stream>>>(p);
+cudaError_t paged_typed(const PagedLaunch& l, cudaStream_t stream) {
+  const dim3 grid((unsigned)((l.p.s.tokens + l.p.perBlock - 1) / l.p.perBlock), l.m.tensors, 1);
+  paged_kernel<VB><<<grid, kPagedThreads, 0, stream>>>(l);
   count_launch();
   return cudaGetLastError();
 }
 
 }  // namespace
 
+// Tokens of a block.
+constexpr int kBlockTokens = 1024;
+// With the pool updated in place: up to this many tokens a cluster, above two kernels.  Measured:
+// 8192 tokens 6.1 against 7.4 us, 131072 tokens 12.6 against 6.8 us.
+constexpr int kClusterTokens = 16384;
+
 cudaError_t launch_pages_build(const PagesBuild& b, const int* poolIn, int* poolOut, int* tokenOffset, int* pageOffset,
-                               int, cudaStream_t stream) {
-  pages_one_block<<<1, 1024, 0, stream>>>(b, poolIn, poolOut, tokenOffset, pageOffset);
+                               int numSM, cudaStream_t stream) {
+  const bool inPlace = b.freeList && poolIn == poolOut;
+  if (b.s.requests <= kSharedRequests && (!inPlace || b.s.maxTokens <= kClusterTokens)) {
+    int blocks = 1;
+    const int most = inPlace ? kMostBlocks : numSM;
+    while (blocks * 2 <= most && b.s.maxTokens > blocks * kBlockTokens) blocks *= 2;
+    if (inPlace && blocks > 8) {
+      const cudaError_t e = cudaFuncSetAttribute(pages_build, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+      if (e != cudaSuccess) return e;
+    }
+    cudaLaunchAttribute cluster{};
+    cluster.id = cudaLaunchAttributeClusterDimension;
+    cluster.val.clusterDim.x = blocks;
+    cluster.val.clusterDim.y = 1;
+    cluster.val.clusterDim.z = 1;
+    cudaLaunchConfig_t c{};
+    c.gridDim = dim3(blocks);
+    c.blockDim = dim3(b.s.requests > 512 || b.s.maxTokens > 512 ? 1024 : 512);
+    c.dynamicSmemBytes = 8 * (b.s.requests + 1);
+    c.stream = stream;
+    c.attrs = &cluster;
+    c.numAttrs = inPlace ? 1 : 0;
+    const cudaError_t e = cudaLaunchKernelEx(&c, pages_build, b, poolIn, poolOut, tokenOffset, pageOffset, inPlace);
+    if (e == cudaSuccess) count_launch();
+    return e;
+  }
+  pages_scan<<<1, 1024, 0, stream>>>(b, poolIn, poolOut, tokenOffset, pageOffset);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
   count_launch();
-  return cudaGetLastError();
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t c{};
+  const int want = (b.s.maxTokens + kExpandThreads - 1) / kExpandThreads;
+  c.gridDim = dim3(want < numSM * 8 ? want : numSM * 8);
+  c.blockDim = dim3(kExpandThreads);
+  c.stream = stream;
+  c.attrs = &attr;
+  c.numAttrs = 1;
+  e = cudaLaunchKernelEx(&c, pages_expand, b);
+  if (e == cudaSuccess) count_launch();
+  return e;
 }
 
-cudaError_t launch_paged(const PagedShape& s, const PagedMove& m, int, cudaStream_t stream) {
+cudaError_t launch_paged(const PagedShape& s, const PagedMove& m, cudaStream_t stream) {
   if (s.tokens == 0) return cudaSuccess;
-  PagedLaunch p;
-  p.s = s;
-  p.m = m;
-  p.divPage = make_fastdiv(s.pageSize);
-  unsigned long long bits = (unsigned long long)s.headSize * s.elt | (unsigned long long)m.tokenStride |
-                            (unsigned long long)m.headStride | (unsigned long long)(s.pageStride * s.elt) |
-                            (unsigned long long)(s.slotStride * s.elt) | (unsigned long long)(s.headStride * s.elt);
-  for (int i = 0; i < m.tensors; i++) bits |= (uintptr_t)m.src[i] | (uintptr_t)m.dst[i];
-  switch (access_bytes(bits, s.elt)) {
-    case 16: return paged_vec<16>(p, stream);
-    case 8: return paged_vec<8>(p, stream);
-    case 4: return paged_vec<4>(p, stream);
-    case 2: return paged_vec<2>(p, stream);
-    default: return paged_vec<1>(p, stream);
+  unsigned long long addresses = 0;
+  for (int i = 0; i < m.tensors; i++) addresses |= (uintptr_t)m.src[i] | (uintptr_t)m.dst[i];
+  const PagedLaunch l{paged_items(s, m.tokenStride, m.headStride, addresses), m};
+  switch (l.p.access) {
+    case 16: return paged_typed<16>(l, stream);
+    case 8: return paged_typed<8>(l, stream);
+    case 4: return paged_typed<4>(l, stream);
+    case 2: return paged_typed<2>(l, stream);
+    default: return paged_typed<1>(l, stream);
   }
 }
 

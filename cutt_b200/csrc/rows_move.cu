@@ -18,13 +18,6 @@ namespace cuttb {
 
 namespace {
 
-template <int VB> struct Raw;
-template <> struct Raw<16> { typedef uint4 T; };
-template <> struct Raw<8> { typedef uint2 T; };
-template <> struct Raw<4> { typedef uint32_t T; };
-template <> struct Raw<2> { typedef uint16_t T; };
-template <> struct Raw<1> { typedef uint8_t T; };
-
 __device__ __forceinline__ float to_f(float x) { return x; }
 __device__ __forceinline__ float to_f(__half x) { return __half2float(x); }
 __device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
@@ -35,192 +28,382 @@ template <> __device__ __forceinline__ __half from_f<__half>(float x) { return _
 template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 template <> __device__ __forceinline__ uint8_t from_f<uint8_t>(float) { return 0; }
 
-// VB bytes as elements.
-template <typename T, int VB>
+// 16 bytes as elements.
+template <typename T>
 union Piece {
-  static constexpr int N = VB / (int)sizeof(T);
-  typename Raw<VB>::T raw;
+  static constexpr int N = 16 / (int)sizeof(T);
+  uint4 raw;
+  uint32_t w[4];
   T e[N];
   __device__ Piece() {}
 };
 
-template <int TEAM>
-__device__ __forceinline__ float team_sum(float v, float* s) {
-  for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
-  if (TEAM == 32) return v;
-  const int w = threadIdx.x >> 5;
-  if ((threadIdx.x & 31) == 0) s[w] = v;
-  __syncthreads();
-  float t = 0.f;
-  for (int i = 0; i < TEAM / 32; i++) t += s[i];
-  __syncthreads();
-  return t;
+// 16 bytes that start m bytes (0 .. 15) into the 32 of x and y.
+__device__ __forceinline__ uint4 shift_bytes(const uint4& x, const uint4& y, int m) {
+  uint32_t w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+  if (m & 8) {
+#pragma unroll
+    for (int i = 0; i < 6; i++) w[i] = w[i + 2];
+  }
+  if (m & 4) {
+#pragma unroll
+    for (int i = 0; i < 5; i++) w[i] = w[i + 1];
+  }
+  const int sh = (m & 3) * 8;
+  return make_uint4(__funnelshift_r(w[0], w[1], sh), __funnelshift_r(w[1], w[2], sh), __funnelshift_r(w[2], w[3], sh),
+                    __funnelshift_r(w[3], w[4], sh));
+}
+
+// Rows are marked as not to be used again (ld.cs, st.cs): most moves are larger than the cache, and
+// lines so marked make room for one another.  Gradients of 16384 tokens, 4 KB rows, half of 8 slots
+// each dropped: 182 instead of 200 us; sums of 1024 x 8 rows 15.7 instead of 17.5.
+__device__ __forceinline__ uint4 load_16(const unsigned char* a) { return __ldcs((const uint4*)a); }
+__device__ __forceinline__ void store_16(unsigned char* a, const uint4& v) { __stcs((uint4*)a, v); }
+
+// Rows at any address.  Bytes lo .. lo+15 of a row lie in two aligned 16-byte words.  Where lo grows
+// by 16 from lane to lane, the second word is the first of the lane above: every lane loads one and
+// gets the other by shuffle, and the last lane has no piece of its own.  (Both words loaded by every
+// lane need twice the registers: sums over 8 rows of 2001 bf16 for 16384 tokens took 245 us that
+// way, 163 this way.)
+//
+// The word in which byte lo lies: a single access if it lies in the tensor, which `near` (the row
+// is within 16 bytes of the tensor's ends) tells; else, and beyond the row, what the row has of it.
+__device__ __forceinline__ bool near_end(long long row, long long rows, long long stride) {
+  return row * stride < 16 || (rows - 1 - row) * stride < 16;
+}
+template <typename T>
+__device__ __forceinline__ uint4 load_word(const unsigned char* row, int lo, int bytes, bool near) {
+  const int at = lo - (int)((uintptr_t)(row + lo) & 15);          // where the word begins, from the row's start
+  Piece<T> p;
+  p.raw = make_uint4(0, 0, 0, 0);
+  if (at < bytes && at > -16) {
+    if (!near || (at >= 0 && at + 16 <= bytes)) {
+      p.raw = load_16(row + at);
+    } else {
+#pragma unroll
+      for (int i = 0; i < p.N; i++) {
+        const int e = at + i * (int)sizeof(T);
+        if (e >= 0 && e < bytes) p.e[i] = *(const T*)(row + e);
+      }
+    }
+  }
+  return p.raw;
+}
+// The word of the lane above (d = 1) or below (d = -1).
+__device__ __forceinline__ uint4 word_of(const uint4& w, int d) {
+  uint4 r;
+  if (d > 0) {
+    r.x = __shfl_down_sync(0xffffffffu, w.x, 1);
+    r.y = __shfl_down_sync(0xffffffffu, w.y, 1);
+    r.z = __shfl_down_sync(0xffffffffu, w.z, 1);
+    r.w = __shfl_down_sync(0xffffffffu, w.w, 1);
+  } else {
+    r.x = __shfl_up_sync(0xffffffffu, w.x, 1);
+    r.y = __shfl_up_sync(0xffffffffu, w.y, 1);
+    r.z = __shfl_up_sync(0xffffffffu, w.z, 1);
+    r.w = __shfl_up_sync(0xffffffffu, w.w, 1);
+  }
+  return r;
+}
+// The piece from this lane's word and the next one's.
+__device__ __forceinline__ uint4 join_words(const uint4& w, const unsigned char* row, int lo) {
+  return shift_bytes(w, word_of(w, 1), (int)((uintptr_t)(row + lo) & 15));
+}
+// Elements that are not the row's own become zero (they count in sums along the row).
+template <typename T>
+__device__ __forceinline__ void clear_outside(Piece<T>& p, int lo, int bytes) {
+  if (lo >= 0 && lo + 16 <= bytes) return;
+#pragma unroll
+  for (int i = 0; i < p.N; i++) {
+    const int at = lo + i * (int)sizeof(T);
+    if (at < 0 || at >= bytes) p.e[i] = from_f<T>(0.f);
+  }
+}
+
+// Stores a piece that starts on a 16-byte boundary: all of it, or the elements that are the row's own.
+template <typename T>
+__device__ __forceinline__ void store_any(const Piece<T>& p, unsigned char* row, int lo, int bytes) {
+  if (lo >= 0 && lo + 16 <= bytes) {
+    store_16(row + lo, p.raw);
+  } else {
+#pragma unroll
+    for (int i = 0; i < p.N; i++) {
+      const int at = lo + i * (int)sizeof(T);
+      if (at >= 0 && at < bytes) *(T*)(row + at) = p.e[i];
+    }
+  }
 }
 
 constexpr int kThreads = 256;
 constexpr int kPadBlocks = 4;    // blocks per expert that clear padding rows
 
+// Sums K values over a team and writes value j to dweight[j], j < n.  Within a warp every step
+// halves the values a lane holds (K / 2 + K / 4 + .. shuffles, then one per step): lane l ends with
+// value l * K / 32.
+template <int K, int TEAM>
+__device__ __forceinline__ void team_sums(float (&v)[K], float* dweight, int n, float (*part)[K]) {
+  const int lane = threadIdx.x & 31;
+  int d = 16;
+#pragma unroll
+  for (int h = K / 2; h >= 1; h >>= 1, d >>= 1) {
+    const bool up = lane & d;
+#pragma unroll
+    for (int i = 0; i < h; i++) {
+      const float keep = up ? v[i + h] : v[i], send = up ? v[i] : v[i + h];
+      v[i] = keep + __shfl_xor_sync(0xffffffffu, send, d);
+    }
+  }
+  for (; d >= 1; d >>= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], d);
+  const int j = lane / (32 / K);
+  const bool owner = lane % (32 / K) == 0;
+  if (TEAM == 32) {
+    if (owner && j < n) dweight[j] = v[0];
+  } else {
+    if (owner) part[threadIdx.x >> 5][j] = v[0];
+    __syncthreads();
+    if ((int)threadIdx.x < K && (int)threadIdx.x < n) {
+      float t = 0.f;
+#pragma unroll
+      for (int i = 0; i < TEAM / 32; i++) t += part[i][threadIdx.x];
+      dweight[threadIdx.x] = t;
+    }
+    __syncthreads();
+  }
+}
+
+// Rows (-1: dropped) and weights of the slots j0 .. j0+KU-1 of a token.
+template <int KU>
+__device__ __forceinline__ void load_slots(const RowsMove& m, long long s0, int j0, int (&row)[KU], float (&w)[KU]) {
+#pragma unroll
+  for (int j = 0; j < KU; j++) {
+    row[j] = j0 + j < m.choices ? m.rowOf[s0 + j0 + j] : -1;
+    if ((unsigned)row[j] >= (unsigned)m.capacity) row[j] = -1;
+  }
+#pragma unroll
+  for (int j = 0; j < KU; j++) w[j] = m.weight && row[j] >= 0 ? m.weight[s0 + j0 + j] : 1.f;
+}
+
+template <int KU>
+__device__ __forceinline__ bool near_rows(const RowsMove& m, const int (&row)[KU]) {
+  bool near = false;
+#pragma unroll
+  for (int j = 0; j < KU; j++) near = near || (row[j] >= 0 && near_end(row[j], m.capacity, m.rowStride));
+  return near;
+}
+
+// Blocks that an SM is to hold: more registers where a thread keeps many rows' words, else more warps.
+constexpr int scatter_blocks(bool any, bool dot) { return dot ? (any ? 2 : 3) : any ? 8 : 4; }
+constexpr int gather_blocks(bool any, int ku) { return ku > 4 ? 3 : 4; }
+
+// ANY: rows at any address; the pieces of a row are then cut at the 16-byte boundaries of the row
+// that is written, so its first and last pieces may be partial.  The token's words are cut at its
+// own boundaries; a piece lies in the lane's word and that of the lane below or above, so the first
+// and the last lane have no pieces.
+//
 // grid.x: blocks of padding (experts * kPadBlocks of them, or none), then blocks of teams;
 // grid.y: parts of a row.
-template <typename T, int VB, int KU, int TEAM, bool WEIGHT, bool DOT>
-__global__ void __launch_bounds__(kThreads) scatter_kernel(const __grid_constant__ RowsMove m, int padBlocks) {
-  typedef typename Raw<VB>::T R;
-  __shared__ float scratch[kThreads / 32];
-  const int vecs = m.width * (int)sizeof(T) / VB;
-  const int part = (vecs + gridDim.y - 1) / gridDim.y;
-  const int v0 = blockIdx.y * part, v1 = min(vecs, v0 + part);
+template <typename T, bool ANY, int KU, int TEAM, bool WEIGHT, bool DOT>
+__global__ void __launch_bounds__(kThreads, scatter_blocks(ANY, DOT))
+scatter_kernel(const __grid_constant__ RowsMove m, int padBlocks) {
+  __shared__ float part[kThreads / 32][KU];
+  const int bytes = m.width * (int)sizeof(T);
+  const int vecs = bytes / 16 + (ANY ? 2 : 0);
+  const int share = (vecs + gridDim.y - 1) / gridDim.y;
+  const int v0 = blockIdx.y * share, v1 = min(vecs, v0 + share);
   if ((int)blockIdx.x < padBlocks) {
     const int e = blockIdx.x / kPadBlocks;
     const int from = m.offset[e] + m.count[e], to = min(m.offset[e + 1], m.capacity);
-    R zero = {};
+    Piece<T> zero;
+    zero.raw = make_uint4(0, 0, 0, 0);
     for (int r = max(0, from) + blockIdx.x % kPadBlocks; r < to; r += kPadBlocks) {
-      R* y = (R*)(m.row + (long long)r * m.rowStride);
-      for (int v = v0 + threadIdx.x; v < v1; v += kThreads) y[v] = zero;
+      unsigned char* y = const_cast<unsigned char*>(m.row) + (long long)r * m.rowStride;
+      const int mis = ANY ? (int)((uintptr_t)y & 15) : 0;
+      for (int v = v0 + threadIdx.x; v < v1; v += kThreads) {
+        if (ANY) store_any(zero, y, v * 16 - mis, bytes);
+        else store_16(y + v * 16, zero.raw);
+      }
     }
     return;
   }
+  constexpr int STEP = ANY ? TEAM / 32 * 30 : TEAM;
   const int lane = threadIdx.x % TEAM;
+  const int first = ANY ? lane / 32 * 30 + lane % 32 - 1 : lane;
+  const bool lender = ANY && (lane % 32 == 0 || lane % 32 == 31);
   const int t = (blockIdx.x - padBlocks) * (kThreads / TEAM) + threadIdx.x / TEAM;
   if (t >= m.tokens) return;      // whole teams leave
-  const R* x = (const R*)(m.token + (long long)t * m.tokenStride);
+  const unsigned char* x = m.token + (long long)t * m.tokenStride;
+  const int misX = ANY ? (int)((uintptr_t)x & 15) : 0;
+  const bool nearX = ANY && near_end(t, m.tokens, m.tokenStride);
   const long long s0 = (long long)t * m.choices;
   for (int j0 = 0; j0 < m.choices; j0 += KU) {
     int row[KU];
     float w[KU], dot[KU];
+    load_slots<KU>(m, s0, j0, row, w);
 #pragma unroll
-    for (int j = 0; j < KU; j++) {
-      row[j] = j0 + j < m.choices ? m.rowOf[s0 + j0 + j] : -1;
-      if ((unsigned)row[j] >= (unsigned)m.capacity) row[j] = -1;
-      w[j] = WEIGHT && row[j] >= 0 ? m.weight[s0 + j0 + j] : 1.f;
-      dot[j] = 0.f;
-    }
-    for (int v = v0 + lane; v < v1; v += TEAM) {
-      Piece<T, VB> a, o[DOT ? KU : 1];
-      a.raw = x[v];
+    for (int j = 0; j < KU; j++) dot[j] = 0.f;
+    for (int v = v0 + first; ANY ? __any_sync(0xffffffffu, !lender && v < v1) : v < v1; v += STEP) {
+      Piece<T> a, o[DOT ? KU : 1];
+      uint4 below, here, above;
+      if (ANY) here = load_word<T>(x, v * 16 - misX, bytes, nearX);
+      else a.raw = load_16(x + v * 16);
       if (DOT) {
 #pragma unroll
-        for (int j = 0; j < KU; j++)
-          if (row[j] >= 0) o[j].raw = ((const R*)(m.other + (long long)row[j] * m.otherStride))[v];
+        for (int j = 0; j < KU; j++) {
+          if (row[j] < 0) continue;
+          const unsigned char* z = m.other + (long long)row[j] * m.otherStride;
+          if (ANY) {
+            const int lo = v * 16 - (int)((uintptr_t)(m.row + (long long)row[j] * m.rowStride) & 15);
+            o[DOT ? j : 0].raw = load_word<T>(z, lo, bytes, near_end(row[j], m.capacity, m.otherStride));
+          } else {
+            o[DOT ? j : 0].raw = load_16(z + v * 16);
+          }
+        }
+      }
+      if (ANY) {
+        below = word_of(here, -1);
+        above = word_of(here, 1);
       }
 #pragma unroll
       for (int j = 0; j < KU; j++) {
-        if (row[j] < 0) continue;
-        Piece<T, VB> b;
+        if (row[j] < 0) continue;                                  // the same for all lanes
+        unsigned char* y = const_cast<unsigned char*>(m.row) + (long long)row[j] * m.rowStride;
+        const int misY = ANY ? (int)((uintptr_t)y & 15) : 0;
+        const int lo = v * 16 - misY;
+        if (ANY) {
+          if (DOT) o[DOT ? j : 0].raw = join_words(o[DOT ? j : 0].raw, m.other + (long long)row[j] * m.otherStride, lo);
+          a.raw = misX >= misY ? shift_bytes(here, above, misX - misY) : shift_bytes(below, here, 16 + misX - misY);
+          if (lender || v >= v1 || lo >= bytes) continue;
+          if (DOT) {
+            clear_outside(a, lo, bytes);
+            clear_outside(o[DOT ? j : 0], lo, bytes);
+          }
+        }
+        Piece<T> b;
         if (WEIGHT) {
 #pragma unroll
           for (int i = 0; i < b.N; i++) b.e[i] = from_f<T>(to_f(a.e[i]) * w[j]);
         } else {
           b.raw = a.raw;
         }
-        ((R*)(m.row + (long long)row[j] * m.rowStride))[v] = b.raw;
+        if (ANY) store_any(b, y, lo, bytes);
+        else store_16(y + lo, b.raw);
         if (DOT) {
 #pragma unroll
           for (int i = 0; i < b.N; i++) dot[j] = fmaf(to_f(a.e[i]), to_f(o[DOT ? j : 0].e[i]), dot[j]);
         }
       }
     }
-    if (DOT) {
-#pragma unroll
-      for (int j = 0; j < KU; j++) {
-        const float d = team_sum<TEAM>(dot[j], scratch);
-        if (lane == 0 && j0 + j < m.choices) m.dweight[s0 + j0 + j] = d;
-      }
-    }
+    if (DOT) team_sums<KU, TEAM>(dot, m.dweight + s0 + j0, m.choices - j0, part);
   }
 }
 
-template <typename T, int VB, int KU, int TEAM, bool WEIGHT, bool DOT>
-__global__ void __launch_bounds__(kThreads) gather_kernel(const __grid_constant__ RowsMove m) {
-  typedef typename Raw<VB>::T R;
-  __shared__ float scratch[kThreads / 32];
-  const int vecs = m.width * (int)sizeof(T) / VB;
-  const int part = (vecs + gridDim.y - 1) / gridDim.y;
-  const int v0 = blockIdx.y * part, v1 = min(vecs, v0 + part);
+template <typename T, bool ANY, int KU, int TEAM, bool DOT>
+__global__ void __launch_bounds__(kThreads, gather_blocks(ANY, KU))
+gather_kernel(const __grid_constant__ RowsMove m) {
+  __shared__ float part[kThreads / 32][KU];
+  constexpr int N = Piece<T>::N;
+  // pieces that a team takes at once: with ANY the last lane of every warp only lends its bytes
+  constexpr int STEP = ANY ? TEAM / 32 * 31 : TEAM;
+  const int bytes = m.width * (int)sizeof(T);
+  const int vecs = bytes / 16 + (ANY ? 2 : 0);
+  const int share = (vecs + gridDim.y - 1) / gridDim.y;
+  const int v0 = blockIdx.y * share, v1 = min(vecs, v0 + share);
   const int lane = threadIdx.x % TEAM;
+  const int first = ANY ? lane - lane / 32 : lane;
+  const bool lender = ANY && lane % 32 == 31;
   const int t = blockIdx.x * (kThreads / TEAM) + threadIdx.x / TEAM;
   if (t >= m.tokens) return;
-  R* out = (R*)(m.token + (long long)t * m.tokenStride);
-  const R* x = (const R*)(m.other + (long long)t * m.otherStride);
+  unsigned char* out = const_cast<unsigned char*>(m.token) + (long long)t * m.tokenStride;
+  const unsigned char* x = m.other + (long long)t * m.otherStride;
+  const int mis = ANY ? (int)((uintptr_t)out & 15) : 0;
+  const bool nearX = ANY && DOT && near_end(t, m.tokens, m.otherStride);
   const long long s0 = (long long)t * m.choices;
-  // More choices than KU: the slots are gone through in groups, and a thread keeps the sum of its
-  // access in registers over all groups (one access at a time); the weights' gradient is taken
-  // group by group.
+  // Up to KU choices: one walk over the row does everything.  More: the weights' gradient takes a
+  // walk for each group of KU slots, then one walk sums over all groups in registers.
   const bool one = m.choices <= KU;
-  for (int j0 = 0; j0 < m.choices; j0 += KU) {
-    int row[KU];
-    float w[KU], dot[KU];
+  int row[KU];
+  float w[KU];
+  bool near = false;
+  if (one || DOT) {
+    for (int j0 = 0; j0 < m.choices; j0 += KU) {
+      float dot[KU];
+      load_slots<KU>(m, s0, j0, row, w);
+      if (ANY) near = near_rows<KU>(m, row);
 #pragma unroll
-    for (int j = 0; j < KU; j++) {
-      row[j] = j0 + j < m.choices ? m.rowOf[s0 + j0 + j] : -1;
-      if ((unsigned)row[j] >= (unsigned)m.capacity) row[j] = -1;
-      w[j] = WEIGHT && row[j] >= 0 ? m.weight[s0 + j0 + j] : 1.f;
-      dot[j] = 0.f;
-    }
-    if (one || DOT) {
-      for (int v = v0 + lane; v < v1; v += TEAM) {
-        Piece<T, VB> b[KU], a;
-        float sum[Piece<T, VB>::N];
+      for (int j = 0; j < KU; j++) dot[j] = 0.f;
+      for (int v = v0 + first; ANY ? __any_sync(0xffffffffu, v < v1) : v < v1; v += STEP) {
+        const int lo = v * 16 - mis;
+        Piece<T> b[KU], a;
+        float sum[N];
 #pragma unroll
-        for (int i = 0; i < a.N; i++) sum[i] = 0.f;
-#pragma unroll
-        for (int j = 0; j < KU; j++)
-          if (row[j] >= 0) b[j].raw = ((const R*)(m.row + (long long)row[j] * m.rowStride))[v];
-        if (DOT) a.raw = x[v];
+        for (int i = 0; i < N; i++) sum[i] = 0.f;
 #pragma unroll
         for (int j = 0; j < KU; j++) {
           if (row[j] < 0) continue;
+          const unsigned char* y = m.row + (long long)row[j] * m.rowStride;
+          b[j].raw = ANY ? load_word<T>(y, lo, bytes, near) : load_16(y + lo);
+        }
+        if (DOT) a.raw = ANY ? load_word<T>(x, lo, bytes, nearX) : load_16(x + lo);
+        if (ANY && DOT) a.raw = join_words(a.raw, x, lo);
+        if (ANY) {
 #pragma unroll
-          for (int i = 0; i < a.N; i++) {
+          for (int j = 0; j < KU; j++)
+            if (row[j] >= 0) b[j].raw = join_words(b[j].raw, m.row + (long long)row[j] * m.rowStride, lo);
+          if (lender || v >= v1 || lo >= bytes) continue;
+        }
+        if (ANY && DOT) clear_outside(a, lo, bytes);
+#pragma unroll
+        for (int j = 0; j < KU; j++) {
+          if (row[j] < 0) continue;
+          if (ANY && DOT) clear_outside(b[j], lo, bytes);
+#pragma unroll
+          for (int i = 0; i < N; i++) {
             const float f = to_f(b[j].e[i]);
-            sum[i] = WEIGHT ? fmaf(w[j], f, sum[i]) : sum[i] + f;
+            sum[i] = fmaf(w[j], f, sum[i]);
             if (DOT) dot[j] = fmaf(f, to_f(a.e[i]), dot[j]);
           }
         }
         if (one) {
-          Piece<T, VB> r;
+          Piece<T> r;
 #pragma unroll
-          for (int i = 0; i < r.N; i++) r.e[i] = from_f<T>(sum[i]);
-          out[v] = r.raw;
+          for (int i = 0; i < N; i++) r.e[i] = from_f<T>(sum[i]);
+          if (ANY) store_any(r, out, lo, bytes);
+          else store_16(out + lo, r.raw);
         }
       }
-    }
-    if (DOT) {
-#pragma unroll
-      for (int j = 0; j < KU; j++) {
-        const float d = team_sum<TEAM>(dot[j], scratch);
-        if (lane == 0 && j0 + j < m.choices) m.dweight[s0 + j0 + j] = d;
-      }
+      if (DOT) team_sums<KU, TEAM>(dot, m.dweight + s0 + j0, m.choices - j0, part);
     }
   }
   if (one) return;
-  for (int v = v0 + lane; v < v1; v += TEAM) {
-    float sum[Piece<T, VB>::N];
+  for (int v = v0 + first; ANY ? __any_sync(0xffffffffu, v < v1) : v < v1; v += STEP) {
+    const int lo = v * 16 - mis;
+    float sum[N];
 #pragma unroll
-    for (int i = 0; i < Piece<T, VB>::N; i++) sum[i] = 0.f;
+    for (int i = 0; i < N; i++) sum[i] = 0.f;
     for (int j0 = 0; j0 < m.choices; j0 += KU) {
-      Piece<T, VB> b[KU];
-      int row[KU];
+      Piece<T> b[KU];
+      load_slots<KU>(m, s0, j0, row, w);
+      if (ANY) near = near_rows<KU>(m, row);
 #pragma unroll
       for (int j = 0; j < KU; j++) {
-        row[j] = j0 + j < m.choices ? m.rowOf[s0 + j0 + j] : -1;
-        if ((unsigned)row[j] >= (unsigned)m.capacity) row[j] = -1;
-        if (row[j] >= 0) b[j].raw = ((const R*)(m.row + (long long)row[j] * m.rowStride))[v];
+        if (row[j] < 0) continue;
+        const unsigned char* y = m.row + (long long)row[j] * m.rowStride;
+        b[j].raw = ANY ? load_word<T>(y, lo, bytes, near) : load_16(y + lo);
       }
 #pragma unroll
       for (int j = 0; j < KU; j++) {
         if (row[j] < 0) continue;
-        const float w = WEIGHT ? m.weight[s0 + j0 + j] : 1.f;
+        if (ANY) b[j].raw = join_words(b[j].raw, m.row + (long long)row[j] * m.rowStride, lo);
 #pragma unroll
-        for (int i = 0; i < b[j].N; i++) {
-          const float f = to_f(b[j].e[i]);
-          sum[i] = WEIGHT ? fmaf(w, f, sum[i]) : sum[i] + f;
-        }
+        for (int i = 0; i < N; i++) sum[i] = fmaf(w[j], to_f(b[j].e[i]), sum[i]);
       }
     }
-    Piece<T, VB> r;
+    if (ANY && (lender || v >= v1 || lo >= bytes)) continue;
+    Piece<T> r;
 #pragma unroll
-    for (int i = 0; i < r.N; i++) r.e[i] = from_f<T>(sum[i]);
-    out[v] = r.raw;
+    for (int i = 0; i < N; i++) r.e[i] = from_f<T>(sum[i]);
+    if (ANY) store_any(r, out, lo, bytes);
+    else store_16(out + lo, r.raw);
   }
 }
 
@@ -229,67 +412,70 @@ struct Shape {
   int team;
 };
 
-// A warp per token where that fills the GPU; else a block per token, and (where no sum runs along
-// the row) several blocks.
-Shape shape_for(const RowsMove& m, int vecs, bool dot, int numSM) {
+// A block per token, and several where there are few tokens and no sum runs along the row; a warp
+// per token for sums over rows and along them, where tokens are enough to fill the GPU (32 warps per
+// SM).  Measured (bf16): 16384 tokens to 8 rows of 8 KB, block 211 us, warp 236; 16384 sums of 8
+// rows of 8 KB, block 214, warp 190; gradients of both with half the slots dropped, 4 KB, block
+// 130 and 73, warp 116 and 63.
+Shape shape_for(const RowsMove& m, int vecs, bool scatter, int numSM) {
   Shape s;
-  const long long warps = m.tokens;
-  s.team = warps >= (long long)numSM * 32 ? 32 : kThreads;
+  const bool dot = m.dweight != nullptr;
+  s.team = (dot || !scatter) && m.tokens >= numSM * 32 ? 32 : kThreads;
   const int perBlock = kThreads / s.team;
   s.grid = dim3((unsigned)((m.tokens + perBlock - 1) / perBlock), 1, 1);
-  if (!dot && s.team == kThreads) {
-    int parts = (vecs + kThreads - 1) / kThreads;
-    if (parts > 8) parts = 8;
-    s.grid.y = parts;
+  if (!dot && m.tokens < numSM * 8) {
+    const int parts = (vecs + kThreads - 1) / kThreads;
+    s.grid.y = parts < 8 ? parts : 8;
   }
   return s;
 }
 
-template <typename T, int VB, int KU, int TEAM>
-void scatter_flags(const RowsMove& m, dim3 grid, int pad, cudaStream_t stream) {
-  const bool w = m.weight != nullptr, d = m.dweight != nullptr;
-  if (sizeof(T) == 1) {
-    scatter_kernel<T, VB, KU, TEAM, false, false><<<grid, kThreads, 0, stream>>>(m, pad);
-    return;
+template <typename T, bool ANY, int KU>
+void scatter_flags(const RowsMove& m, int team, dim3 grid, int pad, cudaStream_t stream) {
+  const bool w = m.weight != nullptr;
+  if constexpr (sizeof(T) > 1) {
+    if (m.dweight && team == 32) {
+      if (w) scatter_kernel<T, ANY, KU, 32, true, true><<<grid, kThreads, 0, stream>>>(m, pad);
+      else scatter_kernel<T, ANY, KU, 32, false, true><<<grid, kThreads, 0, stream>>>(m, pad);
+      return;
+    }
+    if (m.dweight) {
+      if (w) scatter_kernel<T, ANY, KU, kThreads, true, true><<<grid, kThreads, 0, stream>>>(m, pad);
+      else scatter_kernel<T, ANY, KU, kThreads, false, true><<<grid, kThreads, 0, stream>>>(m, pad);
+      return;
+    }
+    if (w) {
+      scatter_kernel<T, ANY, KU, kThreads, true, false><<<grid, kThreads, 0, stream>>>(m, pad);
+      return;
+    }
   }
-  if (w && d) scatter_kernel<T, VB, KU, TEAM, true, true><<<grid, kThreads, 0, stream>>>(m, pad);
-  else if (w) scatter_kernel<T, VB, KU, TEAM, true, false><<<grid, kThreads, 0, stream>>>(m, pad);
-  else if (d) scatter_kernel<T, VB, KU, TEAM, false, true><<<grid, kThreads, 0, stream>>>(m, pad);
-  else scatter_kernel<T, VB, KU, TEAM, false, false><<<grid, kThreads, 0, stream>>>(m, pad);
+  scatter_kernel<T, ANY, KU, kThreads, false, false><<<grid, kThreads, 0, stream>>>(m, pad);
 }
 
-template <typename T, int VB, int KU, int TEAM>
+template <typename T, bool ANY, int KU, int TEAM>
 void gather_flags(const RowsMove& m, dim3 grid, cudaStream_t stream) {
-  const bool w = m.weight != nullptr, d = m.dweight != nullptr;
-  if (w && d) gather_kernel<T, VB, KU, TEAM, true, true><<<grid, kThreads, 0, stream>>>(m);
-  else if (w) gather_kernel<T, VB, KU, TEAM, true, false><<<grid, kThreads, 0, stream>>>(m);
-  else if (d) gather_kernel<T, VB, KU, TEAM, false, true><<<grid, kThreads, 0, stream>>>(m);
-  else gather_kernel<T, VB, KU, TEAM, false, false><<<grid, kThreads, 0, stream>>>(m);
+  if (m.dweight) gather_kernel<T, ANY, KU, TEAM, true><<<grid, kThreads, 0, stream>>>(m);
+  else gather_kernel<T, ANY, KU, TEAM, false><<<grid, kThreads, 0, stream>>>(m);
 }
 
-template <typename T, int VB>
+template <typename T, bool ANY>
 cudaError_t move_vec(const RowsMove& m, bool scatter, int pad, int numSM, cudaStream_t stream) {
-  const Shape s = shape_for(m, m.width * (int)sizeof(T) / VB, m.dweight != nullptr, numSM);
+  const Shape s = shape_for(m, m.width * (int)sizeof(T) / 16 + (ANY ? 2 : 0), scatter, numSM);
   dim3 g = s.grid;
   if (scatter) {
     g.x += pad;
     if (g.x == 0) return cudaSuccess;
-    if (s.team == 32) {
-      if (m.choices <= 4) scatter_flags<T, VB, 4, 32>(m, g, pad, stream);
-      else scatter_flags<T, VB, 8, 32>(m, g, pad, stream);
-    } else {
-      if (m.choices <= 4) scatter_flags<T, VB, 4, kThreads>(m, g, pad, stream);
-      else scatter_flags<T, VB, 8, kThreads>(m, g, pad, stream);
-    }
+    if (m.choices <= 4) scatter_flags<T, ANY, 4>(m, s.team, g, pad, stream);
+    else scatter_flags<T, ANY, 8>(m, s.team, g, pad, stream);
   } else {
     if (g.x == 0) return cudaSuccess;
     if constexpr (sizeof(T) > 1) {
       if (s.team == 32) {
-        if (m.choices <= 4) gather_flags<T, VB, 4, 32>(m, g, stream);
-        else gather_flags<T, VB, 8, 32>(m, g, stream);
+        if (m.choices <= 4) gather_flags<T, ANY, 4, 32>(m, g, stream);
+        else gather_flags<T, ANY, 8, 32>(m, g, stream);
       } else {
-        if (m.choices <= 4) gather_flags<T, VB, 4, kThreads>(m, g, stream);
-        else gather_flags<T, VB, 8, kThreads>(m, g, stream);
+        if (m.choices <= 4) gather_flags<T, ANY, 4, kThreads>(m, g, stream);
+        else gather_flags<T, ANY, 8, kThreads>(m, g, stream);
       }
     }
   }
@@ -302,8 +488,8 @@ cudaError_t move_typed(const RowsMove& m, bool scatter, int pad, int numSM, cuda
   unsigned long long bits = (uintptr_t)m.token | (uintptr_t)m.row | (uintptr_t)m.other | (unsigned long long)m.tokenStride |
                             (unsigned long long)m.rowStride | (unsigned long long)(m.width * (long long)sizeof(T));
   if (m.other) bits |= (unsigned long long)m.otherStride;
-  if (access_bytes(bits, sizeof(T)) == 16) return move_vec<T, 16>(m, scatter, pad, numSM, stream);
-  return move_vec<T, sizeof(T)>(m, scatter, pad, numSM, stream);
+  if (bits % 16 == 0) return move_vec<T, false>(m, scatter, pad, numSM, stream);
+  return move_vec<T, true>(m, scatter, pad, numSM, stream);
 }
 
 cudaError_t move(const RowsMove& m, bool scatter, int pad, int numSM, cudaStream_t stream) {

@@ -133,4 +133,27 @@ int access_bytes(unsigned long long bits, int elt) {
   return vb;
 }
 
+PagedItems paged_items(const PagedShape& s, long long tokenStride, long long headStride, unsigned long long addresses) {
+  PagedItems p;
+  p.s = s;
+  p.tokenStride = tokenStride;
+  p.headStride = headStride;
+  // longer pieces, and wider accesses where the head size is odd
+  if (s.headStride == s.headSize && headStride == (long long)s.headSize * s.elt) {
+    p.s.headSize = s.headSize * s.heads;
+    p.s.heads = 1;
+  }
+  unsigned long long bits = addresses | (unsigned long long)p.s.headSize * s.elt | (unsigned long long)tokenStride |
+                            (unsigned long long)(s.pageStride * s.elt) | (unsigned long long)(s.slotStride * s.elt);
+  if (p.s.heads > 1) bits |= (unsigned long long)headStride | (unsigned long long)(s.headStride * s.elt);
+  p.access = access_bytes(bits, s.elt);
+  const int perHead = p.s.headSize * s.elt / p.access;
+  p.vecs = perHead * p.s.heads;
+  p.divPage = make_fastdiv(s.pageSize);
+  p.divHead = make_fastdiv(perHead);
+  p.divRow = make_fastdiv(p.vecs);
+  p.perBlock = p.vecs >= kPagedThreads * kPagedItems ? 1 : kPagedThreads * kPagedItems / p.vecs;
+  return p;
+}
+
 }  // namespace cuttb

@@ -69,6 +69,9 @@ int access_bytes(unsigned long long bits, int elt);
 CUTT_HD int local_expert(long long e, int first, int experts) {
   return e >= first && e < (long long)first + experts ? (int)(e - first) : -1;
 }
+CUTT_HD int local_expert(int e, int first, int experts) {
+  return e >= first && e < first + experts ? e - first : -1;     // first + experts fits: check_rows_shape
+}
 
 // Segment of an expert with n rows that starts at row o (not clipped): what fits into `capacity`.
 CUTT_HD int clip_row(int o, int capacity) { return o < capacity ? o : capacity; }
@@ -146,6 +149,33 @@ CUTT_HD long long cache_offset(const PagedShape& s, long long slot, const FastDi
   }
   const uint32_t page = fdiv((uint32_t)slot, divPage);
   return page * s.pageStride + ((uint32_t)slot - page * (uint32_t)s.pageSize) * s.slotStride;
+}
+
+// Rows stored into or loaded from pages, as accesses of `access` bytes.
+struct PagedItems {
+  PagedShape s;                        // heads that lie one behind the other on both sides are one
+  long long tokenStride, headStride;   // of the rows, bytes
+  int access;
+  int vecs;                            // accesses of a token
+  int perBlock;                        // tokens of a block
+  FastDiv divPage, divRow, divHead;    // by pageSize, by accesses of a token, by accesses of a head
+};
+constexpr int kPagedThreads = 256;
+constexpr int kPagedItems = 4;         // accesses of a thread in flight at once
+
+// strides in bytes; addresses: those of all rows and caches, or-ed together.
+PagedItems paged_items(const PagedShape& s, long long tokenStride, long long headStride, unsigned long long addresses);
+
+// Access i of a block whose first token is q0: byte offsets in the cache and in the rows.  False where
+// the token's slot is not one of the cache's.
+CUTT_HD bool paged_item(const PagedItems& p, const long long* slot, int q0, uint32_t i, long long& cache, long long& row) {
+  const uint32_t q = fdiv(i, p.divRow), r = i - q * (uint32_t)p.vecs;
+  const uint32_t h = fdiv(r, p.divHead), v = r - h * p.divHead.d;
+  const long long at = cache_offset(p.s, slot[q0 + q], p.divPage);
+  if (at < 0) return false;
+  cache = (at + (long long)h * p.s.headStride) * p.s.elt + (long long)v * p.access;
+  row = (long long)(q0 + q) * p.tokenStride + (long long)h * p.headStride + (long long)v * p.access;
+  return true;
 }
 
 }  // namespace cuttb

@@ -26,9 +26,9 @@ class Build:
         return plain_build(self.held.tolist(), self.added.tolist(), page, width, self.free.tolist() if take else None,
                            self.pool.tolist(), self.table.tolist(), m)
 
-    def build(self):
+    def build(self, pool_out=None):
         self.plan.build(self.held.data_ptr(), self.added.data_ptr(), self.free.data_ptr(), self.pool.data_ptr(),
-                        self.pool.data_ptr(), self.table.data_ptr(), self.tokens.data_ptr(), self.pages.data_ptr(),
+                        (self.pool if pool_out is None else pool_out).data_ptr(), self.table.data_ptr(), self.tokens.data_ptr(), self.pages.data_ptr(),
                         self.slot.data_ptr(), table_stride=self.table.stride(0))
 
     def check(self, want):
@@ -58,7 +58,12 @@ def test_build(native, b, page, width, decode):
     for spare, short, extra in ((3, 0, 0), (0, max(1, need // 3), 2), (-1, 0, 0)):
         n = 5 + max(0, need - short)
         c = Build(native, held, added, page, width, list(range(7000, 7000 + n)), [5, n], max(0, total + spare), extra)
-        want = c.want()
+        want, table = c.want(), c.table.clone()
+        apart = c.torch.zeros_like(c.pool)
+        c.build(apart)                                       # into another pool, then in place
+        assert apart.tolist() == want[4] and c.table.tolist() == want[0] and c.slot.tolist() == want[3] + [-7] * 4
+        c.table.copy_(table)
+        c.slot.fill_(-7)
         c.build()
         c.check(want)
         # the same lengths over the table as it is now, without taking pages
@@ -70,8 +75,9 @@ def test_build(native, b, page, width, decode):
         assert c.slot.tolist() == want[3] + [-7] * 4 and c.table.tolist() == want[0] and c.tokens.tolist() == want[1]
 
 
-@pytest.mark.parametrize("b,m", [(1, 300000), (300, 200000), (40, 65537)])
-def test_build_of_long_steps(native, b, m):
+@pytest.mark.parametrize("in_place", [True, False])
+@pytest.mark.parametrize("b,m", [(1, 300000), (300, 200000), (40, 65537), (5000, 30000), (4096, 5000), (7, 16384), (7, 16385)])
+def test_build_of_long_steps(native, b, m, in_place):
     import random
     rng = random.Random(m)
     cut = sorted(rng.randint(0, m - 100) for _ in range(b - 1))
@@ -82,7 +88,12 @@ def test_build_of_long_steps(native, b, m):
     n = sum(-(-(h + a) // page) for h, a in zip(held, added)) + 1
     c = Build(native, held, added, page, width, rng.sample(range(10 * n), n), [0, n], m)
     want = c.want()
-    c.build()
+    before = c.pool.clone()
+    out = c.pool if in_place else c.torch.zeros_like(c.pool)
+    c.build(out)
+    if not in_place:
+        assert c.torch.equal(c.pool, before)
+        c.pool = out
     c.check(want)
 
 

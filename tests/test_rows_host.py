@@ -28,6 +28,8 @@ def hc(native):
     L.cutt_hostcheck_pages_run.restype = ll
     L.cutt_hostcheck_cache_offset.argtypes = [i, i, ll, ll, ll]
     L.cutt_hostcheck_cache_offset.restype = ll
+    L.cutt_hostcheck_paged_run.argtypes = [vp, vp, ll, ll, vp, vp, ll, vp, ll, i]
+    L.cutt_hostcheck_paged_run.restype = ll
     L.cutt_hostcheck_local_expert.argtypes = [ll, i, i]
     return L
 
@@ -281,3 +283,46 @@ def test_local_expert(hc):
     assert [f(e, 4, 3) for e in (-1, 3, 4, 6, 7)] == [-1, -1, 0, 2, -1]
     for e in (2**63 - 1, -2**63, 2**32 + 4, 2**31):
         assert f(e, 4, 3) == -1
+
+
+@pytest.mark.parametrize("elt", [1, 2, 4, 8])
+@pytest.mark.parametrize("heads,size,page,head_major,pad,shift", [
+    (8, 128, 16, True, 0, 0), (1, 64, 1, False, 0, 0), (3, 33, 24, True, 0, 1), (2, 80, 64, False, 5, 0), (5, 1, 7, True, 1, 0),
+    (1, 576, 64, False, 0, 0), (40, 128, 16, False, 0, 0), (8, 33, 16, False, 0, 0), (8, 33, 16, False, 0, 3), (3, 700, 4, False, 0, 0)])
+def test_paged_accesses_on_the_host(hc, elt, heads, size, page, head_major, pad, shift):
+    """Every access of the store and load kernels: inside the buffers, aligned, and the right element."""
+    rng = np.random.default_rng(heads * 1000 + size)
+    pages, n = 11, min(90, 11 * page - 3)
+    wide = size + pad
+    dt = {1: np.uint8, 2: np.uint16, 4: np.uint32, 8: np.uint64}[elt]
+
+    def buffer(count):
+        raw = np.zeros(count * elt + 64, np.uint8)
+        at = -raw.ctypes.data % 16 + shift * elt
+        return raw, raw[at:at + count * elt].view(dt)
+
+    shape = (pages, heads, page, wide) if head_major else (pages, page, heads, wide)
+    keep, flat = buffer(int(np.prod(shape)))
+    flat[:] = rng.integers(0, 250, flat.size)
+    keep2, rows = buffer(n * heads * wide)
+    rows[:] = rng.integers(0, 250, rows.size)
+    cache = flat.reshape(shape)
+    view = cache.transpose(0, 2, 1, 3) if head_major else cache            # page, place, head, element
+    strides = (ctypes.c_longlong * 3)(*[view.strides[k] // elt for k in (0, 1, 2)])
+    slot = rng.permutation(pages * page)[:n].astype(np.int64)
+    slot[::7] = -1
+    slot[1], slot[2] = pages * page, 2**40
+    live = [(q, s) for q, s in enumerate(slot.tolist()) if 0 <= s < pages * page]
+    ints = _ints(n, heads, size, elt, pages, page)
+    r3 = rows.reshape(n, heads, wide)
+    for store in (1, 0):
+        want_cache, want_rows = view.copy(), r3.copy()
+        for q, s in live:
+            if store:
+                want_cache[s // page, s % page, :, :size] = r3[q, :, :size]
+            else:
+                want_rows[q, :, :size] = view[s // page, s % page, :, :size]
+        assert hc.cutt_hostcheck_paged_run(ints, strides, heads * wide, wide, slot.ctypes.data, rows.ctypes.data, rows.nbytes,
+                                           flat.ctypes.data, flat.nbytes, store) == 0
+        assert np.array_equal(view, want_cache) and np.array_equal(r3, want_rows)
+        rows[:] = rng.integers(0, 250, rows.size)
