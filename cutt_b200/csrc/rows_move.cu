@@ -3,10 +3,14 @@
 // dispatch), with the gradient of the weights on the way.
 //
 // Both walk over tokens, so the token side is read or written once and the k-fold side once: the
-// fewest bytes there are.  A team of threads (a warp, or a block where there are few tokens) owns a
-// token, or a part of its row; every thread holds one access of the token's row and goes through
-// the token's slots.  Sums are in 32 bits in the order of the slots, rounded once, so results do
-// not depend on the launch shape.
+// fewest bytes there are.  A block owns a token, or a part of its row; every thread holds one access
+// of the token's row and goes through the token's slots.  Sums are in 32 bits in the order of the
+// slots, rounded once, so results do not depend on the launch shape.
+//
+// What bounds them is memory: 16384 tokens to 8 rows of 8 KB (bf16) take 188 us, 6.4 TB/s, which is
+// what a copy reaches.  Blocks of one token that end soon, many of them on an SM, do best: teams that
+// stay and go over the tokens with the next one's slots prefetched took 238 us there, and a warp for a
+// token 236.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <stdint.h>
@@ -134,14 +138,13 @@ __device__ __forceinline__ void store_any(const Piece<T>& p, unsigned char* row,
   }
 }
 
-constexpr int kThreads = 256;
 constexpr int kPadBlocks = 4;    // blocks per expert that clear padding rows
 
-// Sums K values over a team and writes value j to dweight[j], j < n.  Within a warp every step
+// Sums K values over the block and writes value j to dweight[j], j < n.  Within a warp every step
 // halves the values a lane holds (K / 2 + K / 4 + .. shuffles, then one per step): lane l ends with
 // value l * K / 32.
-template <int K, int TEAM>
-__device__ __forceinline__ void team_sums(float (&v)[K], float* dweight, int n, float (*part)[K]) {
+template <int K, int THREADS>
+__device__ __forceinline__ void block_sums(float (&v)[K], float* dweight, int n, float (*part)[K]) {
   const int lane = threadIdx.x & 31;
   int d = 16;
 #pragma unroll
@@ -154,21 +157,15 @@ __device__ __forceinline__ void team_sums(float (&v)[K], float* dweight, int n, 
     }
   }
   for (; d >= 1; d >>= 1) v[0] += __shfl_xor_sync(0xffffffffu, v[0], d);
-  const int j = lane / (32 / K);
-  const bool owner = lane % (32 / K) == 0;
-  if (TEAM == 32) {
-    if (owner && j < n) dweight[j] = v[0];
-  } else {
-    if (owner) part[threadIdx.x >> 5][j] = v[0];
-    __syncthreads();
-    if ((int)threadIdx.x < K && (int)threadIdx.x < n) {
-      float t = 0.f;
+  if (lane % (32 / K) == 0) part[threadIdx.x >> 5][lane / (32 / K)] = v[0];
+  __syncthreads();
+  if ((int)threadIdx.x < K && (int)threadIdx.x < n) {
+    float t = 0.f;
 #pragma unroll
-      for (int i = 0; i < TEAM / 32; i++) t += part[i][threadIdx.x];
-      dweight[threadIdx.x] = t;
-    }
-    __syncthreads();
+    for (int i = 0; i < THREADS / 32; i++) t += part[i][threadIdx.x];
+    dweight[threadIdx.x] = t;
   }
+  __syncthreads();
 }
 
 // Rows (-1: dropped) and weights of the slots j0 .. j0+KU-1 of a token.
@@ -191,21 +188,25 @@ __device__ __forceinline__ bool near_rows(const RowsMove& m, const int (&row)[KU
   return near;
 }
 
-// Blocks that an SM is to hold: more registers where a thread keeps many rows' words, else more warps.
-constexpr int scatter_blocks(bool any, bool dot) { return dot ? (any ? 2 : 3) : any ? 8 : 4; }
-constexpr int gather_blocks(bool any, int ku) { return ku > 4 ? 3 : 4; }
+// Warps that an SM is to hold at least, which limits a thread's registers.  A thread that keeps the
+// pieces of many rows needs registers, the others do better with more warps.  Measured, us: rows out
+// with the weights' gradient (16384 tokens, half of 8 slots dropped, 4 KB) 24 warps 110, 32 warps 124;
+// 16384 tokens to 8 rows of 2001 bf16 with 32, 48, 64 warps 119, 126, 132; sums of 8 rows of 4 KB, half
+// dropped, 24, 28, 32 warps 60, 57, 59; sums of 4 rows of 5 KB 32, 40, 48 warps 36.2, 35.2, 35.5.
+constexpr int scatter_warps(bool any, bool dot) { return dot ? (any ? 16 : 24) : 32; }
+constexpr int gather_warps(int ku) { return ku > 4 ? 28 : 40; }
 
 // ANY: rows at any address; the pieces of a row are then cut at the 16-byte boundaries of the row
 // that is written, so its first and last pieces may be partial.  The token's words are cut at its
 // own boundaries; a piece lies in the lane's word and that of the lane below or above, so the first
 // and the last lane have no pieces.
 //
-// grid.x: blocks of padding (experts * kPadBlocks of them, or none), then blocks of teams;
-// grid.y: parts of a row.
-template <typename T, bool ANY, int KU, int TEAM, bool WEIGHT, bool DOT>
-__global__ void __launch_bounds__(kThreads, scatter_blocks(ANY, DOT))
+// grid.x: blocks of padding (experts * kPadBlocks of them, or none), then one for each token; grid.y:
+// parts of a row.
+template <typename T, bool ANY, int KU, int THREADS, bool WEIGHT, bool DOT>
+__global__ void __launch_bounds__(THREADS, scatter_warps(ANY, DOT) * 32 / THREADS)
 scatter_kernel(const __grid_constant__ RowsMove m, int padBlocks) {
-  __shared__ float part[kThreads / 32][KU];
+  __shared__ float part[THREADS / 32][KU];
   const int bytes = m.width * (int)sizeof(T);
   const int vecs = bytes / 16 + (ANY ? 2 : 0);
   const int share = (vecs + gridDim.y - 1) / gridDim.y;
@@ -218,19 +219,18 @@ scatter_kernel(const __grid_constant__ RowsMove m, int padBlocks) {
     for (int r = max(0, from) + blockIdx.x % kPadBlocks; r < to; r += kPadBlocks) {
       unsigned char* y = const_cast<unsigned char*>(m.row) + (long long)r * m.rowStride;
       const int mis = ANY ? (int)((uintptr_t)y & 15) : 0;
-      for (int v = v0 + threadIdx.x; v < v1; v += kThreads) {
+      for (int v = v0 + threadIdx.x; v < v1; v += THREADS) {
         if (ANY) store_any(zero, y, v * 16 - mis, bytes);
         else store_16(y + v * 16, zero.raw);
       }
     }
     return;
   }
-  constexpr int STEP = ANY ? TEAM / 32 * 30 : TEAM;
-  const int lane = threadIdx.x % TEAM;
+  constexpr int STEP = ANY ? THREADS / 32 * 30 : THREADS;
+  const int lane = threadIdx.x;
   const int first = ANY ? lane / 32 * 30 + lane % 32 - 1 : lane;
   const bool lender = ANY && (lane % 32 == 0 || lane % 32 == 31);
-  const int t = (blockIdx.x - padBlocks) * (kThreads / TEAM) + threadIdx.x / TEAM;
-  if (t >= m.tokens) return;      // whole teams leave
+  const int t = blockIdx.x - padBlocks;
   const unsigned char* x = m.token + (long long)t * m.tokenStride;
   const int misX = ANY ? (int)((uintptr_t)x & 15) : 0;
   const bool nearX = ANY && near_end(t, m.tokens, m.tokenStride);
@@ -293,26 +293,25 @@ scatter_kernel(const __grid_constant__ RowsMove m, int padBlocks) {
         }
       }
     }
-    if (DOT) team_sums<KU, TEAM>(dot, m.dweight + s0 + j0, m.choices - j0, part);
+    if (DOT) block_sums<KU, THREADS>(dot, m.dweight + s0 + j0, m.choices - j0, part);
   }
 }
 
-template <typename T, bool ANY, int KU, int TEAM, bool DOT>
-__global__ void __launch_bounds__(kThreads, gather_blocks(ANY, KU))
+template <typename T, bool ANY, int KU, int THREADS, bool DOT>
+__global__ void __launch_bounds__(THREADS, gather_warps(KU) * 32 / THREADS)
 gather_kernel(const __grid_constant__ RowsMove m) {
-  __shared__ float part[kThreads / 32][KU];
+  __shared__ float part[THREADS / 32][KU];
   constexpr int N = Piece<T>::N;
-  // pieces that a team takes at once: with ANY the last lane of every warp only lends its bytes
-  constexpr int STEP = ANY ? TEAM / 32 * 31 : TEAM;
+  // pieces that the block takes at once: with ANY the last lane of every warp only lends its bytes
+  constexpr int STEP = ANY ? THREADS / 32 * 31 : THREADS;
   const int bytes = m.width * (int)sizeof(T);
   const int vecs = bytes / 16 + (ANY ? 2 : 0);
   const int share = (vecs + gridDim.y - 1) / gridDim.y;
   const int v0 = blockIdx.y * share, v1 = min(vecs, v0 + share);
-  const int lane = threadIdx.x % TEAM;
+  const int lane = threadIdx.x;
   const int first = ANY ? lane - lane / 32 : lane;
   const bool lender = ANY && lane % 32 == 31;
-  const int t = blockIdx.x * (kThreads / TEAM) + threadIdx.x / TEAM;
-  if (t >= m.tokens) return;
+  const int t = blockIdx.x;
   unsigned char* out = const_cast<unsigned char*>(m.token) + (long long)t * m.tokenStride;
   const unsigned char* x = m.other + (long long)t * m.otherStride;
   const int mis = ANY ? (int)((uintptr_t)out & 15) : 0;
@@ -371,7 +370,7 @@ gather_kernel(const __grid_constant__ RowsMove m) {
           else store_16(out + lo, r.raw);
         }
       }
-      if (DOT) team_sums<KU, TEAM>(dot, m.dweight + s0 + j0, m.choices - j0, part);
+      if (DOT) block_sums<KU, THREADS>(dot, m.dweight + s0 + j0, m.choices - j0, part);
     }
   }
   if (one) return;
@@ -407,97 +406,121 @@ gather_kernel(const __grid_constant__ RowsMove m) {
   }
 }
 
-struct Shape {
-  dim3 grid;
-  int team;
-};
+// Threads of a token's block.  Measured with 16384 tokens in bf16, us with 64, 128, 256 and 512 threads:
+//   to 8 rows of 8 KB      209, 200, 195, 188      to 2 rows of 8 KB      70,  70,  75,  98
+//   to 4 rows of 8 KB      110, 107, 107, 126      to 8 rows of 2 KB      51,  49,  49,  64
+// so a thread is to have at least 8 stores.  With weights it needs registers, and 512 threads took 201
+// where 256 took 193.
+int scatter_threads(long long pieces, bool weight) {
+  if (pieces >= 8 * 512 && !weight) return 512;
+  return pieces >= 8 * 256 ? 256 : pieces >= 8 * 128 ? 128 : 64;
+}
+// The gradient of the weights with it (64, 128, 256 threads): 8 rows of 8 KB 370, 360, 360; half of them
+// dropped 198, 197, 211; 8 rows of 4 KB 184, 179, 186; half dropped 100, 103, 119; 2 KB 92, 92, 121.  Sums: 8 rows of 8 KB 178, 174, 176; half of 8 rows
+// of 4 KB dropped 57, 61, 75; 8 rows of 2 KB 40, 44, 62.
+// Few tokens (less than 8 for an SM): with a sum along the row that one block has to make, the more
+// threads the better (256 tokens, 8 rows of 8 KB: 16, 11.3, 9.7; 13.1, 9.0, 7.3); without one, several
+// blocks of 128 threads share a row.
+constexpr int kFewTokens = 8;            // for an SM
+constexpr int kMostParts = 8;
 
-// A block per token, and several where there are few tokens and no sum runs along the row; a warp
-// per token for sums over rows and along them, where tokens are enough to fill the GPU (32 warps per
-// SM).  Measured (bf16): 16384 tokens to 8 rows of 8 KB, block 211 us, warp 236; 16384 sums of 8
-// rows of 8 KB, block 214, warp 190; gradients of both with half the slots dropped, 4 KB, block
-// 130 and 73, warp 116 and 63.
-Shape shape_for(const RowsMove& m, int vecs, bool scatter, int numSM) {
-  Shape s;
-  const bool dot = m.dweight != nullptr;
-  s.team = (dot || !scatter) && m.tokens >= numSM * 32 ? 32 : kThreads;
-  const int perBlock = kThreads / s.team;
-  s.grid = dim3((unsigned)((m.tokens + perBlock - 1) / perBlock), 1, 1);
-  if (!dot && m.tokens < numSM * 8) {
-    const int parts = (vecs + kThreads - 1) / kThreads;
-    s.grid.y = parts < 8 ? parts : 8;
+dim3 token_grid(const RowsMove& m, int vecs, int threads, bool few) {
+  dim3 g(m.tokens, 1, 1);
+  if (few && !m.dweight) {
+    const int parts = (vecs + threads - 1) / threads;
+    g.y = parts < kMostParts ? parts : kMostParts;
   }
-  return s;
+  return g;
+}
+
+template <typename T, bool ANY, int KU, int THREADS>
+void run_scatter_dot(const RowsMove& m, dim3 grid, int pad, cudaStream_t stream) {
+  if (m.weight) scatter_kernel<T, ANY, KU, THREADS, true, true><<<grid, THREADS, 0, stream>>>(m, pad);
+  else scatter_kernel<T, ANY, KU, THREADS, false, true><<<grid, THREADS, 0, stream>>>(m, pad);
+}
+
+template <typename T, bool ANY, int KU, int THREADS>
+void run_scatter(const RowsMove& m, dim3 grid, int pad, cudaStream_t stream) {
+  if constexpr (sizeof(T) > 1 && THREADS <= 256) {
+    if (m.weight) {
+      scatter_kernel<T, ANY, KU, THREADS, true, false><<<grid, THREADS, 0, stream>>>(m, pad);
+      return;
+    }
+  }
+  scatter_kernel<T, ANY, KU, THREADS, false, false><<<grid, THREADS, 0, stream>>>(m, pad);
 }
 
 template <typename T, bool ANY, int KU>
-void scatter_flags(const RowsMove& m, int team, dim3 grid, int pad, cudaStream_t stream) {
-  const bool w = m.weight != nullptr;
+void scatter(const RowsMove& m, int pad, int numSM, cudaStream_t stream) {
+  const int vecs = m.width * (int)sizeof(T) / 16 + (ANY ? 2 : 0);
+  const bool few = m.tokens < numSM * kFewTokens;
   if constexpr (sizeof(T) > 1) {
-    if (m.dweight && team == 32) {
-      if (w) scatter_kernel<T, ANY, KU, 32, true, true><<<grid, kThreads, 0, stream>>>(m, pad);
-      else scatter_kernel<T, ANY, KU, 32, false, true><<<grid, kThreads, 0, stream>>>(m, pad);
-      return;
-    }
     if (m.dweight) {
-      if (w) scatter_kernel<T, ANY, KU, kThreads, true, true><<<grid, kThreads, 0, stream>>>(m, pad);
-      else scatter_kernel<T, ANY, KU, kThreads, false, true><<<grid, kThreads, 0, stream>>>(m, pad);
-      return;
-    }
-    if (w) {
-      scatter_kernel<T, ANY, KU, kThreads, true, false><<<grid, kThreads, 0, stream>>>(m, pad);
+      const int threads = few ? 256 : vecs > 256 ? 128 : 64;
+      dim3 g = token_grid(m, vecs, threads, few);
+      g.x += pad;
+      if (threads == 256) run_scatter_dot<T, ANY, KU, 256>(m, g, pad, stream);
+      else if (threads == 128) run_scatter_dot<T, ANY, KU, 128>(m, g, pad, stream);
+      else run_scatter_dot<T, ANY, KU, 64>(m, g, pad, stream);
       return;
     }
   }
-  scatter_kernel<T, ANY, KU, kThreads, false, false><<<grid, kThreads, 0, stream>>>(m, pad);
+  const int threads = few ? 128 : scatter_threads((long long)m.choices * vecs, m.weight != nullptr);
+  dim3 g = token_grid(m, vecs, threads, few);
+  g.x += pad;
+  if (threads == 512) run_scatter<T, ANY, KU, 512>(m, g, pad, stream);
+  else if (threads == 256) run_scatter<T, ANY, KU, 256>(m, g, pad, stream);
+  else if (threads == 128) run_scatter<T, ANY, KU, 128>(m, g, pad, stream);
+  else run_scatter<T, ANY, KU, 64>(m, g, pad, stream);
 }
 
-template <typename T, bool ANY, int KU, int TEAM>
-void gather_flags(const RowsMove& m, dim3 grid, cudaStream_t stream) {
-  if (m.dweight) gather_kernel<T, ANY, KU, TEAM, true><<<grid, kThreads, 0, stream>>>(m);
-  else gather_kernel<T, ANY, KU, TEAM, false><<<grid, kThreads, 0, stream>>>(m);
+template <typename T, bool ANY, int KU, int THREADS>
+void run_gather(const RowsMove& m, dim3 grid, cudaStream_t stream) {
+  if (m.dweight) gather_kernel<T, ANY, KU, THREADS, true><<<grid, THREADS, 0, stream>>>(m);
+  else gather_kernel<T, ANY, KU, THREADS, false><<<grid, THREADS, 0, stream>>>(m);
+}
+
+template <typename T, bool ANY, int KU>
+void gather(const RowsMove& m, int numSM, cudaStream_t stream) {
+  const int vecs = m.width * (int)sizeof(T) / 16 + (ANY ? 2 : 0);
+  const bool few = m.tokens < numSM * kFewTokens;
+  if (few && m.dweight) {
+    gather_kernel<T, ANY, KU, 256, true><<<token_grid(m, vecs, 256, few), 256, 0, stream>>>(m);
+    return;
+  }
+  if (few || vecs >= 512) run_gather<T, ANY, KU, 128>(m, token_grid(m, vecs, 128, few), stream);
+  else run_gather<T, ANY, KU, 64>(m, token_grid(m, vecs, 64, few), stream);
 }
 
 template <typename T, bool ANY>
-cudaError_t move_vec(const RowsMove& m, bool scatter, int pad, int numSM, cudaStream_t stream) {
-  const Shape s = shape_for(m, m.width * (int)sizeof(T) / 16 + (ANY ? 2 : 0), scatter, numSM);
-  dim3 g = s.grid;
-  if (scatter) {
-    g.x += pad;
-    if (g.x == 0) return cudaSuccess;
-    if (m.choices <= 4) scatter_flags<T, ANY, 4>(m, s.team, g, pad, stream);
-    else scatter_flags<T, ANY, 8>(m, s.team, g, pad, stream);
-  } else {
-    if (g.x == 0) return cudaSuccess;
-    if constexpr (sizeof(T) > 1) {
-      if (s.team == 32) {
-        if (m.choices <= 4) gather_flags<T, ANY, 4, 32>(m, g, stream);
-        else gather_flags<T, ANY, 8, 32>(m, g, stream);
-      } else {
-        if (m.choices <= 4) gather_flags<T, ANY, 4, kThreads>(m, g, stream);
-        else gather_flags<T, ANY, 8, kThreads>(m, g, stream);
-      }
-    }
+void move_rows(const RowsMove& m, bool rowsOut, int pad, int numSM, cudaStream_t stream) {
+  if (rowsOut) {
+    if (m.choices <= 4) scatter<T, ANY, 4>(m, pad, numSM, stream);
+    else scatter<T, ANY, 8>(m, pad, numSM, stream);
+  } else if constexpr (sizeof(T) > 1) {
+    if (m.choices <= 4) gather<T, ANY, 4>(m, numSM, stream);
+    else gather<T, ANY, 8>(m, numSM, stream);
   }
+}
+
+template <typename T>
+cudaError_t move_typed(const RowsMove& m, bool rowsOut, int pad, int numSM, cudaStream_t stream) {
+  if (m.tokens == 0 && pad == 0) return cudaSuccess;
+  unsigned long long bits = (uintptr_t)m.token | (uintptr_t)m.row | (uintptr_t)m.other | (unsigned long long)m.tokenStride |
+                            (unsigned long long)m.rowStride | (unsigned long long)(m.width * (long long)sizeof(T));
+  if (m.other) bits |= (unsigned long long)m.otherStride;
+  if (bits % 16) move_rows<T, true>(m, rowsOut, pad, numSM, stream);
+  else move_rows<T, false>(m, rowsOut, pad, numSM, stream);
   count_launch();
   return cudaGetLastError();
 }
 
-template <typename T>
-cudaError_t move_typed(const RowsMove& m, bool scatter, int pad, int numSM, cudaStream_t stream) {
-  unsigned long long bits = (uintptr_t)m.token | (uintptr_t)m.row | (uintptr_t)m.other | (unsigned long long)m.tokenStride |
-                            (unsigned long long)m.rowStride | (unsigned long long)(m.width * (long long)sizeof(T));
-  if (m.other) bits |= (unsigned long long)m.otherStride;
-  if (bits % 16 == 0) return move_vec<T, false>(m, scatter, pad, numSM, stream);
-  return move_vec<T, true>(m, scatter, pad, numSM, stream);
-}
-
-cudaError_t move(const RowsMove& m, bool scatter, int pad, int numSM, cudaStream_t stream) {
+cudaError_t move(const RowsMove& m, bool rowsOut, int pad, int numSM, cudaStream_t stream) {
   switch (m.type) {
-    case 0: return move_typed<uint8_t>(m, scatter, pad, numSM, stream);
-    case 1: return move_typed<__half>(m, scatter, pad, numSM, stream);
-    case 2: return move_typed<__nv_bfloat16>(m, scatter, pad, numSM, stream);
-    case 3: return move_typed<float>(m, scatter, pad, numSM, stream);
+    case 0: return move_typed<uint8_t>(m, rowsOut, pad, numSM, stream);
+    case 1: return move_typed<__half>(m, rowsOut, pad, numSM, stream);
+    case 2: return move_typed<__nv_bfloat16>(m, rowsOut, pad, numSM, stream);
+    case 3: return move_typed<float>(m, rowsOut, pad, numSM, stream);
   }
   return cudaErrorInvalidValue;
 }
@@ -509,7 +532,7 @@ cudaError_t launch_rows_scatter(const RowsMove& m, int align, int numSM, cudaStr
 }
 
 cudaError_t launch_rows_gather(const RowsMove& m, int numSM, cudaStream_t stream) {
-  return move(m, false, 0, numSM, stream);
+  return m.tokens ? move(m, false, 0, numSM, stream) : cudaSuccess;
 }
 
 }  // namespace cuttb
