@@ -124,6 +124,11 @@ __device__ __forceinline__ void clear_outside(Piece<T>& p, int lo, int bytes) {
   }
 }
 
+// Bytes by which a row starts behind a 16-byte boundary.
+__device__ __forceinline__ int past_boundary(const unsigned char* base, int row, long long stride) {
+  return (int)(((unsigned)(uintptr_t)base + (unsigned)row * (unsigned)stride) & 15u);
+}
+
 // Stores a piece that starts on a 16-byte boundary: all of it, or the elements that are the row's own.
 template <typename T>
 __device__ __forceinline__ void store_any(const Piece<T>& p, unsigned char* row, int lo, int bytes) {
@@ -181,10 +186,10 @@ __device__ __forceinline__ void load_slots(const RowsMove& m, long long s0, int 
 }
 
 template <int KU>
-__device__ __forceinline__ bool near_rows(const RowsMove& m, const int (&row)[KU]) {
+__device__ __forceinline__ bool near_rows(const RowsMove& m, const int (&row)[KU], long long stride) {
   bool near = false;
 #pragma unroll
-  for (int j = 0; j < KU; j++) near = near || (row[j] >= 0 && near_end(row[j], m.capacity, m.rowStride));
+  for (int j = 0; j < KU; j++) near = near || (row[j] >= 0 && near_end(row[j], m.capacity, stride));
   return near;
 }
 
@@ -239,6 +244,7 @@ scatter_kernel(const __grid_constant__ RowsMove m, int padBlocks) {
     int row[KU];
     float w[KU], dot[KU];
     load_slots<KU>(m, s0, j0, row, w);
+    const bool nearOther = ANY && DOT && near_rows<KU>(m, row, m.otherStride);
 #pragma unroll
     for (int j = 0; j < KU; j++) dot[j] = 0.f;
     for (int v = v0 + first; ANY ? __any_sync(0xffffffffu, !lender && v < v1) : v < v1; v += STEP) {
@@ -252,8 +258,8 @@ scatter_kernel(const __grid_constant__ RowsMove m, int padBlocks) {
           if (row[j] < 0) continue;
           const unsigned char* z = m.other + (long long)row[j] * m.otherStride;
           if (ANY) {
-            const int lo = v * 16 - (int)((uintptr_t)(m.row + (long long)row[j] * m.rowStride) & 15);
-            o[DOT ? j : 0].raw = load_word<T>(z, lo, bytes, near_end(row[j], m.capacity, m.otherStride));
+            const int lo = v * 16 - past_boundary(m.row, row[j], m.rowStride);
+            o[DOT ? j : 0].raw = load_word<T>(z, lo, bytes, nearOther);
           } else {
             o[DOT ? j : 0].raw = load_16(z + v * 16);
           }
@@ -267,7 +273,7 @@ scatter_kernel(const __grid_constant__ RowsMove m, int padBlocks) {
       for (int j = 0; j < KU; j++) {
         if (row[j] < 0) continue;                                  // the same for all lanes
         unsigned char* y = const_cast<unsigned char*>(m.row) + (long long)row[j] * m.rowStride;
-        const int misY = ANY ? (int)((uintptr_t)y & 15) : 0;
+        const int misY = ANY ? past_boundary(m.row, row[j], m.rowStride) : 0;
         const int lo = v * 16 - misY;
         if (ANY) {
           if (DOT) o[DOT ? j : 0].raw = join_words(o[DOT ? j : 0].raw, m.other + (long long)row[j] * m.otherStride, lo);
@@ -327,7 +333,7 @@ gather_kernel(const __grid_constant__ RowsMove m) {
     for (int j0 = 0; j0 < m.choices; j0 += KU) {
       float dot[KU];
       load_slots<KU>(m, s0, j0, row, w);
-      if (ANY) near = near_rows<KU>(m, row);
+      if (ANY) near = near_rows<KU>(m, row, m.rowStride);
 #pragma unroll
       for (int j = 0; j < KU; j++) dot[j] = 0.f;
       for (int v = v0 + first; ANY ? __any_sync(0xffffffffu, v < v1) : v < v1; v += STEP) {
@@ -382,7 +388,7 @@ gather_kernel(const __grid_constant__ RowsMove m) {
     for (int j0 = 0; j0 < m.choices; j0 += KU) {
       Piece<T> b[KU];
       load_slots<KU>(m, s0, j0, row, w);
-      if (ANY) near = near_rows<KU>(m, row);
+      if (ANY) near = near_rows<KU>(m, row, m.rowStride);
 #pragma unroll
       for (int j = 0; j < KU; j++) {
         if (row[j] < 0) continue;

@@ -262,6 +262,48 @@ def test_gradients(native, kind, shape):
                 assert (dw == 77).all()
 
 
+@pytest.mark.parametrize("kind", ["bytes", "bf16", "f32"])
+@pytest.mark.parametrize("t,k,h,shift", [(1300, 3, 1111, 0), (1300, 4, 2312, 0), (1200, 8, 4096, 0), (1200, 8, 4096, 3), (1190, 2, 4100, 1),
+                                         (1500, 1, 2048, 0), (2500, 6, 520, 0), (1300, 9, 1023, 0), (300, 8, 8200, 0), (1200, 40, 72, 0)])
+def test_every_launch_shape(native, kind, t, k, h, shift):
+    """Tokens enough for every number of threads of a block; compared on the device in 64 bits."""
+    import torch
+    r = Run(native, routing(t, k, max(8, k // 2), 17, 0.3), h, kind, max(8, k // 2), align=8)
+    r.sort()
+    g = torch.Generator().manual_seed(5)
+    token, rows = r.rows(t, g, 0, shift), r.rows(r.r, g, 0, shift)
+    row = torch.tensor(r.want[2], device="cuda").view(t, k)
+    ok = row >= 0
+    y = torch.full((r.r, h), 77, dtype=r.dtype, device="cuda")
+    r.plan.dispatch(token.data_ptr(), *r.maps(), y.data_ptr())
+    assert torch.equal(y[row[ok]], token[:, None, :].expand(t, k, h)[ok])
+    assert (y[r.want[1][-1]:] == 77).all() and (y[r.padding()] == 0).all()
+    if kind == "bytes":
+        return
+    w = torch.randn(t, k, generator=g).cuda()
+    ts = token.double()
+    parts = torch.where(ok[:, :, None], rows.double()[row.clamp_min(0)], 0.0)
+    dw = torch.full((t, k), 77.0, device="cuda")
+    out = torch.full((t, h), 77, dtype=r.dtype, device="cuda")
+    r.plan.combine(rows.data_ptr(), r.row_of.data_ptr(), out.data_ptr(), weight=w.data_ptr())
+    terms = parts * w.double()[:, :, None]
+    want, size = terms.sum(1).cpu(), terms.abs().sum(1).cpu()
+    close(out, want, size, k, kind)
+    out.fill_(77)
+    r.plan.dispatch_grad(rows.data_ptr(), r.row_of.data_ptr(), out.data_ptr(), weight=w.data_ptr(), x=token.data_ptr(), dweight=dw.data_ptr())
+    close(out, want, size, k, kind)
+    products = parts * ts[:, None, :]
+    want, size = products.sum(2).cpu(), products.abs().sum(2).cpu()
+    close(dw, want, size, h, "f32")
+    dw.fill_(77)
+    y.fill_(77)
+    r.plan.combine_grad(token.data_ptr(), *r.maps(), y.data_ptr(), weight=w.data_ptr(), y=rows.data_ptr(), dweight=dw.data_ptr())
+    close(dw, want, size, h, "f32")
+    want = (ts[:, None, :] * w.double()[:, :, None])[ok].cpu()
+    close(y[row[ok]], want, want.abs(), 1, kind)
+    assert (y[r.want[1][-1]:] == 77).all() and (y[r.padding()] == 0).all()
+
+
 def test_broadcast_inputs(native):
     """Inputs of row stride 0: an expanded gradient, one row for all."""
     import torch
