@@ -198,7 +198,7 @@ __device__ __forceinline__ bool near_rows(const RowsMove& m, const int (&row)[KU
 // with the weights' gradient (16384 tokens, half of 8 slots dropped, 4 KB) 24 warps 110, 32 warps 124;
 // 16384 tokens to 8 rows of 2001 bf16 with 32, 48, 64 warps 119, 126, 132; sums of 8 rows of 4 KB, half
 // dropped, 24, 28, 32 warps 60, 57, 59; sums of 4 rows of 5 KB 32, 40, 48 warps 36.2, 35.2, 35.5.
-constexpr int scatter_warps(bool any, bool dot) { return dot ? (any ? 16 : 24) : 32; }
+constexpr int scatter_warps(bool, bool dot) { return dot ? 24 : 32; }
 constexpr int gather_warps(int ku) { return ku > 4 ? 28 : 40; }
 
 // ANY: rows at any address; the pieces of a row are then cut at the 16-byte boundaries of the row
@@ -424,11 +424,17 @@ int scatter_threads(long long pieces, bool weight) {
 // The gradient of the weights with it (64, 128, 256 threads): 8 rows of 8 KB 370, 360, 360; half of them
 // dropped 198, 197, 211; 8 rows of 4 KB 184, 179, 186; half dropped 100, 103, 119; 2 KB 92, 92, 121.  Sums: 8 rows of 8 KB 178, 174, 176; half of 8 rows
 // of 4 KB dropped 57, 61, 75; 8 rows of 2 KB 40, 44, 62.
-// Few tokens (less than 8 for an SM): with a sum along the row that one block has to make, the more
-// threads the better (256 tokens, 8 rows of 8 KB: 16, 11.3, 9.7; 13.1, 9.0, 7.3); without one, several
-// blocks of 128 threads share a row.
+// Few tokens (less than 8 for an SM): without a sum along the row several blocks of 128 threads share
+// one.  With a sum one block has to make it, and more threads are better (256 tokens, 8 rows of 8 KB:
+// 16, 11.3, 9.7; 13.1, 9.0, 7.3; 1024 tokens 28.4, 28.9, 26.9; 19.1, 18.5, 17.8) unless blocks are
+// many and rows too short for them (1023 tokens, 3 rows of 1111 fp32, 128 threads 8.4, 256 11.0).
 constexpr int kFewTokens = 8;            // for an SM
 constexpr int kMostParts = 8;
+
+int sum_threads(const RowsMove& m, int vecs, int numSM) {
+  const bool few = m.tokens < numSM * kFewTokens;
+  return few && (vecs >= 512 || m.tokens < 2 * numSM) ? 256 : vecs > 256 ? 128 : 64;
+}
 
 dim3 token_grid(const RowsMove& m, int vecs, int threads, bool few) {
   dim3 g(m.tokens, 1, 1);
@@ -460,9 +466,10 @@ template <typename T, bool ANY, int KU>
 void scatter(const RowsMove& m, int pad, int numSM, cudaStream_t stream) {
   const int vecs = m.width * (int)sizeof(T) / 16 + (ANY ? 2 : 0);
   const bool few = m.tokens < numSM * kFewTokens;
-  if constexpr (sizeof(T) > 1) {
+  // (rows at any address: four at a time, see move_rows)
+  if constexpr (sizeof(T) > 1 && !(ANY && KU > 4)) {
     if (m.dweight) {
-      const int threads = few ? 256 : vecs > 256 ? 128 : 64;
+      const int threads = sum_threads(m, vecs, numSM);
       dim3 g = token_grid(m, vecs, threads, few);
       g.x += pad;
       if (threads == 256) run_scatter_dot<T, ANY, KU, 256>(m, g, pad, stream);
@@ -480,28 +487,30 @@ void scatter(const RowsMove& m, int pad, int numSM, cudaStream_t stream) {
   else run_scatter<T, ANY, KU, 64>(m, g, pad, stream);
 }
 
-template <typename T, bool ANY, int KU, int THREADS>
-void run_gather(const RowsMove& m, dim3 grid, cudaStream_t stream) {
-  if (m.dweight) gather_kernel<T, ANY, KU, THREADS, true><<<grid, THREADS, 0, stream>>>(m);
-  else gather_kernel<T, ANY, KU, THREADS, false><<<grid, THREADS, 0, stream>>>(m);
-}
-
 template <typename T, bool ANY, int KU>
 void gather(const RowsMove& m, int numSM, cudaStream_t stream) {
   const int vecs = m.width * (int)sizeof(T) / 16 + (ANY ? 2 : 0);
   const bool few = m.tokens < numSM * kFewTokens;
-  if (few && m.dweight) {
-    gather_kernel<T, ANY, KU, 256, true><<<token_grid(m, vecs, 256, few), 256, 0, stream>>>(m);
+  if (m.dweight) {
+    const int threads = few ? sum_threads(m, vecs, numSM) : vecs >= 512 ? 128 : 64;
+    const dim3 g = token_grid(m, vecs, threads, few);
+    if (threads == 256) gather_kernel<T, ANY, KU, 256, true><<<g, 256, 0, stream>>>(m);
+    else if (threads == 128) gather_kernel<T, ANY, KU, 128, true><<<g, 128, 0, stream>>>(m);
+    else gather_kernel<T, ANY, KU, 64, true><<<g, 64, 0, stream>>>(m);
     return;
   }
-  if (few || vecs >= 512) run_gather<T, ANY, KU, 128>(m, token_grid(m, vecs, 128, few), stream);
-  else run_gather<T, ANY, KU, 64>(m, token_grid(m, vecs, 64, few), stream);
+  const int threads = few || vecs >= 512 ? 128 : 64;
+  const dim3 g = token_grid(m, vecs, threads, few);
+  if (threads == 128) gather_kernel<T, ANY, KU, 128, false><<<g, 128, 0, stream>>>(m);
+  else gather_kernel<T, ANY, KU, 64, false><<<g, 64, 0, stream>>>(m);
 }
 
 template <typename T, bool ANY>
 void move_rows(const RowsMove& m, bool rowsOut, int pad, int numSM, cudaStream_t stream) {
   if (rowsOut) {
-    if (m.choices <= 4) scatter<T, ANY, 4>(m, pad, numSM, stream);
+    // Four or eight of a token's rows at a time.  At any address and with the weights' gradient eight leave
+    // too few registers for enough warps: 16384 tokens, 8 rows of 2001 bf16, 471 us, with four 361.
+    if (m.choices <= 4 || (ANY && m.dweight)) scatter<T, ANY, 4>(m, pad, numSM, stream);
     else scatter<T, ANY, 8>(m, pad, numSM, stream);
   } else if constexpr (sizeof(T) > 1) {
     if (m.choices <= 4) gather<T, ANY, 4>(m, numSM, stream);
