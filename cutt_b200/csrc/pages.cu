@@ -181,9 +181,11 @@ struct PagedLaunch {
 };
 
 // grid.x: groups of perBlock tokens, grid.y: tensors.  A thread's loads are all issued before its first
-// store: with 1, 2, 4 and 8 of them 131072 K and V rows of 2 KB took 222, 197, 193 and 217 us.  Loads
-// and stores marked as not to be used again (ld.cs, st.cs) made that 180, and 8192 rows stored before
-// 131072 are loaded 192 instead of 207: the marked lines make room for one another.
+// store.  Memory bounds it: 131072 K and V rows of 2 KB take 165 us, 6.5 TB/s.  Measured there: blocks of
+// 64, 128, 256, 512 threads with four loads each 166, 165, 182, 224; 128 threads with 6, 8 loads 173, 183;
+// 256 threads with 1, 2, 3 loads 222, 197, 181.  Loads and stores are marked as not to be used again
+// (ld.cs, st.cs): 8192 rows stored before 131072 are loaded 192 instead of 207 us (256 threads), since the
+// marked lines make room for one another.
 template <int VB>
 __global__ void __launch_bounds__(kPagedThreads) paged_kernel(const __grid_constant__ PagedLaunch l) {
   typedef typename Raw<VB>::T R;

@@ -160,7 +160,7 @@ struct PagedItems {
   int perBlock;                        // tokens of a block
   FastDiv divPage, divRow, divHead;    // by pageSize, by accesses of a token, by accesses of a head
 };
-constexpr int kPagedThreads = 256;
+constexpr int kPagedThreads = 128;
 constexpr int kPagedItems = 4;         // accesses of a thread in flight at once
 
 // strides in bytes; addresses: those of all rows and caches, or-ed together.
