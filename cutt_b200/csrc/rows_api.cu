@@ -45,7 +45,7 @@ int add_plan(unsigned int* handle, Plan& p, void* stream) {
   try {
     std::shared_ptr<const Plan> q = std::make_shared<Plan>(p);
     std::lock_guard<std::mutex> lk(g_lock);
-    if (g_next >= kRowsHandleBit) return CUTT_INTERNAL_ERROR;
+    if (g_next >= kRowsHandleBit - 1) return CUTT_INTERNAL_ERROR;      // 0xffffffff stays free
     const unsigned int h = g_next | kRowsHandleBit;
     g_table[h] = std::move(q);
     g_next++;

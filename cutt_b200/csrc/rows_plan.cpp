@@ -94,6 +94,7 @@ int check_pages_build(const PagesShape& s, const void* held, const void* added, 
   const bool take = freeList != nullptr;
   if (take != (poolIn != nullptr) || take != (poolOut != nullptr) || take != (pageOffset != nullptr)) return kBad;
   if (tableStride < s.tableWidth || tableStride > (1LL << 56) / s.requests) return kBad;
+  if (poolIn != poolOut && (uintptr_t)poolIn < (uintptr_t)poolOut + 8 && (uintptr_t)poolOut < (uintptr_t)poolIn + 8) return kBad;
   const void* in[] = {held, added, freeList, poolIn};
   const void* out[] = {table, tokenOffset, pageOffset, slot, poolOut};
   for (const void* o : out) {

@@ -61,34 +61,39 @@ def _package():
     return cutt_b200
 
 
+def _c_ints(what: str, *values: int) -> None:
+    """ctypes would cut larger numbers down to 32 bits."""
+    if not all(-2**31 <= v < 2**31 for v in values):
+        C = _package()
+        raise C.CuttError(C.CUTT_INVALID_PARAMETER, what)
+
+
+# Never a plan's number: calls after destroy() are refused as those of any unknown handle.
+_NONE = 0xffffffff
+
+
 class _Handle:
+    """A plan.  Calls are a few microseconds in all, so the methods below go to the C functions directly."""
     handle = None
+    _h = _NONE
 
     def _made(self, rc: int, handle: ctypes.c_uint) -> None:
         C = _package()
         if rc != C.CUTT_SUCCESS:
             raise C.CuttError(rc, type(self).__name__)
-        self.handle = handle.value
+        self.handle = self._h = handle.value
         self._lib = C.lib()
 
-    def _check(self, rc: int, what: str) -> None:
-        if rc:
-            raise _package().CuttError(rc, what)
-
-    def _live(self) -> int:
-        h = self.handle
-        if h is None:
-            C = _package()
-            raise C.CuttError(C.CUTT_INVALID_PLAN, "destroyed")
-        return h
+    def _failed(self, rc: int, what: str):
+        return _package().CuttError(rc, what)
 
     def describe(self) -> str:
-        return _package().plan_describe(self._live())
+        return _package().plan_describe(self._h)
 
     def destroy(self) -> None:
         if self.handle is not None:
             _package().cuttDestroy(self.handle)
-            self.handle = None
+            self.handle, self._h = None, _NONE
 
     def __del__(self):
         try:
@@ -106,6 +111,7 @@ class RowPlan(_Handle):
         if capacity is None:
             slots = tokens * choices
             capacity = max(1, slots + min(experts, slots) * (align - 1))
+        _c_ints("RowPlan", tokens, choices, experts, first, align, capacity, width, type)
         self.capacity, self.width = capacity, width
         h = ctypes.c_uint(0)
         rc = _package().lib().cutt_rows_plan(ctypes.byref(h), tokens, choices, experts, first, align, capacity,
@@ -113,45 +119,51 @@ class RowPlan(_Handle):
         self._made(rc, h)
 
     def sort(self, expert_of: int, index_bytes: int, count: int, offset: int, row_of: int, slot_of: int) -> None:
-        rc = self._lib.cutt_rows_sort(self._live(), expert_of, index_bytes, count, offset, row_of, slot_of)
-        self._check(rc, "sort")
+        rc = self._lib.cutt_rows_sort(self._h, expert_of, index_bytes, count, offset, row_of, slot_of)
+        if rc:
+            raise self._failed(rc, "sort")
 
     def dispatch(self, x: int, row_of: int, count: int, offset: int, y: int, weight: int = 0,
                  x_stride: int | None = None, y_stride: int | None = None) -> None:
         w = self.width
-        rc = self._lib.cutt_rows_dispatch(self._live(), x, w if x_stride is None else x_stride, row_of, count, offset,
+        rc = self._lib.cutt_rows_dispatch(self._h, x, w if x_stride is None else x_stride, row_of, count, offset,
                                           weight, y, w if y_stride is None else y_stride)
-        self._check(rc, "dispatch")
+        if rc:
+            raise self._failed(rc, "dispatch")
 
     def combine(self, y: int, row_of: int, out: int, weight: int = 0, y_stride: int | None = None,
                 out_stride: int | None = None) -> None:
         w = self.width
-        rc = self._lib.cutt_rows_combine(self._live(), y, w if y_stride is None else y_stride, row_of, weight, out,
+        rc = self._lib.cutt_rows_combine(self._h, y, w if y_stride is None else y_stride, row_of, weight, out,
                                          w if out_stride is None else out_stride)
-        self._check(rc, "combine")
+        if rc:
+            raise self._failed(rc, "combine")
 
     def dispatch_grad(self, dy: int, row_of: int, dx: int, weight: int = 0, x: int = 0, dweight: int = 0,
                       dy_stride: int | None = None, x_stride: int | None = None, dx_stride: int | None = None) -> None:
         w = self.width
-        rc = self._lib.cutt_rows_dispatch_grad(self._live(), dy, w if dy_stride is None else dy_stride, row_of, weight,
+        rc = self._lib.cutt_rows_dispatch_grad(self._h, dy, w if dy_stride is None else dy_stride, row_of, weight,
                                                x, w if x_stride is None else x_stride, dx,
                                                w if dx_stride is None else dx_stride, dweight)
-        self._check(rc, "dispatch_grad")
+        if rc:
+            raise self._failed(rc, "dispatch_grad")
 
     def combine_grad(self, dout: int, row_of: int, count: int, offset: int, dy: int, weight: int = 0, y: int = 0,
                      dweight: int = 0, dout_stride: int | None = None, y_stride: int | None = None,
                      dy_stride: int | None = None) -> None:
         w = self.width
-        rc = self._lib.cutt_rows_combine_grad(self._live(), dout, w if dout_stride is None else dout_stride, row_of,
+        rc = self._lib.cutt_rows_combine_grad(self._h, dout, w if dout_stride is None else dout_stride, row_of,
                                               count, offset, weight, y, w if y_stride is None else y_stride, dy,
                                               w if dy_stride is None else dy_stride, dweight)
-        self._check(rc, "combine_grad")
+        if rc:
+            raise self._failed(rc, "combine_grad")
 
 
 class PagePlan(_Handle):
     """Block tables and slot maps of ``requests`` requests (cutt_pages_plan)."""
 
     def __init__(self, requests: int, page_size: int, table_width: int, max_tokens: int, stream: int = 0):
+        _c_ints("PagePlan", requests, page_size, table_width, max_tokens)
         self.table_width = table_width
         h = ctypes.c_uint(0)
         rc = _package().lib().cutt_pages_plan(ctypes.byref(h), requests, page_size, table_width, max_tokens, stream)
@@ -159,10 +171,11 @@ class PagePlan(_Handle):
 
     def build(self, held: int, added: int, free_list: int, pool_in: int, pool_out: int, table: int, token_offset: int,
               page_offset: int, slot: int, table_stride: int | None = None) -> None:
-        rc = self._lib.cutt_pages_build(self._live(), held, added, free_list, pool_in, pool_out, table,
+        rc = self._lib.cutt_pages_build(self._h, held, added, free_list, pool_in, pool_out, table,
                                         self.table_width if table_stride is None else table_stride, token_offset,
                                         page_offset, slot)
-        self._check(rc, "build")
+        if rc:
+            raise self._failed(rc, "build")
 
     def slots(self, held: int, added: int, table: int, token_offset: int, slot: int, table_stride: int | None = None) -> None:
         """Slots of tokens whose pages the table has already: no page is taken, the table is only read."""
@@ -174,6 +187,7 @@ class PagedRows(_Handle):
 
     def __init__(self, tokens: int, heads: int, head_size: int, element_bytes: int, pages: int, page_size: int,
                  page_stride: int, slot_stride: int, head_stride: int, stream: int = 0):
+        _c_ints("PagedRows", tokens, heads, head_size, element_bytes, pages, page_size)
         self.token_stride, self.head_stride = heads * head_size, head_size
         h = ctypes.c_uint(0)
         rc = _package().lib().cutt_pages_plan_rows(ctypes.byref(h), tokens, heads, head_size, element_bytes, pages,
@@ -182,13 +196,15 @@ class PagedRows(_Handle):
 
     def store(self, k: int, v: int, slot: int, k_cache: int, v_cache: int, token_stride: int | None = None,
               head_stride: int | None = None) -> None:
-        rc = self._lib.cutt_pages_store(self._live(), k, v, self.token_stride if token_stride is None else token_stride,
+        rc = self._lib.cutt_pages_store(self._h, k, v, self.token_stride if token_stride is None else token_stride,
                                         self.head_stride if head_stride is None else head_stride, slot, k_cache, v_cache)
-        self._check(rc, "store")
+        if rc:
+            raise self._failed(rc, "store")
 
     def load(self, k_cache: int, v_cache: int, slot: int, k: int, v: int, token_stride: int | None = None,
              head_stride: int | None = None) -> None:
-        rc = self._lib.cutt_pages_load(self._live(), k_cache, v_cache, slot, k, v,
+        rc = self._lib.cutt_pages_load(self._h, k_cache, v_cache, slot, k, v,
                                        self.token_stride if token_stride is None else token_stride,
                                        self.head_stride if head_stride is None else head_stride)
-        self._check(rc, "load")
+        if rc:
+            raise self._failed(rc, "load")

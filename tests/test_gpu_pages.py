@@ -97,6 +97,30 @@ def test_build_of_long_steps(native, b, m, in_place):
     c.check(want)
 
 
+def test_long_build_captured_with_the_pool_in_place(native):
+    """Two kernels in a CUDA graph; every replay takes pages from where the last one stopped."""
+    import torch
+    side = torch.cuda.Stream()
+    b, m = 9, 20000
+    with torch.cuda.stream(side):
+        c = Build(native, [0] * b, [0] * b, 16, 400, list(range(9000, 9000 + 4000)), [0, 4000], m)
+        c.build()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        c.build()
+    held = [0] * b
+    for added in ([100, 0, 3000, 7, 1, 900, 16, 31, 2], [1] * b, [0] * b, [5000, 1, 1, 0, 0, 3, 2000, 15, 1]):
+        c.held.copy_(torch.tensor(held, dtype=torch.int32))
+        c.added.copy_(torch.tensor(added, dtype=torch.int32))
+        torch.cuda.synchronize()
+        want = c.want()
+        graph.replay()
+        torch.cuda.synchronize()
+        c.check(want)
+        held = [x + y for x, y in zip(held, added)]
+
+
 def test_build_of_empty_and_odd_lengths(native):
     for held, added in (([0, 0, 0], [0, 0, 0]), ([0], [0]), ([-5, 7, -1], [3, -9, 0]), ([100, 32, 31], [5, 1, 2])):
         c = Build(native, held, added, 8, 4, list(range(50, 70)), [2, 20], 9)

@@ -319,6 +319,57 @@ def test_broadcast_inputs(native):
     close(out, 3 * one.double().cpu().expand(50, 64), 3 * one.double().cpu().abs().expand(50, 64), 3, "bf16")
 
 
+@pytest.mark.parametrize("h", [33, 7, 2001])
+def test_broadcast_inputs_at_any_address(native, h):
+    """Row stride 0 and rows that start anywhere: nothing outside the one row is read (its neighbours are NaN
+    and would show)."""
+    import torch
+    r = Run(native, routing(1300, 3, 6, 1), h, "bf16", 6, align=4)
+    r.sort()
+    buf = torch.full((h + 64,), float("nan"), dtype=torch.bfloat16, device="cuda")
+    one = buf[5:5 + h]
+    one.copy_(torch.randn(h))
+    y = torch.zeros(r.r, h, dtype=torch.bfloat16, device="cuda")
+    dw = torch.zeros(1300, 3, device="cuda")
+    w = torch.ones(1300, 3, device="cuda")
+    r.plan.combine_grad(one.data_ptr(), *r.maps(), y.data_ptr(), weight=w.data_ptr(), y=one.data_ptr(), dweight=dw.data_ptr(),
+                        dout_stride=0, y_stride=0)
+    row, ok = r.live()
+    assert torch.equal(y[row[ok].long().cuda()], one.expand(int(ok.sum()), h))
+    square = (one.double() ** 2).sum().cpu()
+    close(dw, square.expand(1300, 3), square.expand(1300, 3), h, "f32")
+    out = torch.zeros(1300, h, dtype=torch.bfloat16, device="cuda")
+    r.plan.dispatch_grad(one.data_ptr(), r.row_of.data_ptr(), out.data_ptr(), x=one.data_ptr(), dweight=dw.data_ptr(), dy_stride=0,
+                         x_stride=0)
+    size = 3 * one.double().cpu().expand(1300, h)
+    close(out, size, size.abs(), 3, "bf16")
+    close(dw, square.expand(1300, 3), square.expand(1300, 3), h, "f32")
+
+
+def test_long_map_captured_and_replayed(native):
+    """The map in three kernels inside a CUDA graph, replayed with other routings; twice the same input gives
+    the same map."""
+    import torch
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        r = Run(native, routing(70000, 2, 200, 1), 8, "bf16", 200, align=16)
+        r.sort()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        r.sort()
+    for seed in (2, 3, 3):
+        ids = routing(70000, 2, 200, seed, 0.2)
+        r.ids.copy_(ids)
+        for t in (r.count, r.offset, r.row_of, r.slot_of):
+            t.fill_(-9)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        r.want = plain_map(ids.reshape(-1).tolist(), 0, 200, 16, r.r)
+        r.check_map()
+
+
 def test_not_a_number_stays_in_its_row(native):
     import torch
     r = Run(native, routing(40, 4, 8, 2), 256, "f32", 8)

@@ -92,6 +92,14 @@ def test_paged_plan_refusals(native, hc, change):
     assert native.lib().cutt_pages_plan_rows(ctypes.byref(h), *bad.values(), None) == BAD
 
 
+def test_numbers_beyond_32_bits_are_refused_in_python(native):
+    for make in (lambda: native.RowPlan(2**32 + 4, 1, 8, 16, 2), lambda: native.RowPlan(4, 1, 8, 2**32 + 16, 2),
+                 lambda: native.PagePlan(1, 2**32 + 1, 4, 4), lambda: native.PagedRows(4, 1, 8, 2, 2**32 + 2, 8, 64, 8, 8)):
+        with pytest.raises(native.CuttError) as e:
+            make()
+        assert e.value.code == BAD
+
+
 def test_calls_on_unknown_handles(native):
     L = native.lib()
     for h in (0x80000000 + 12345, 3, 0xffffffff):
@@ -165,7 +173,7 @@ def test_build_refusals(hc):
     assert rc(free=0, poolIn=0, poolOut=0, pageOffset=0) == 0
     for change in (dict(held=0), dict(added=0), dict(table=0), dict(tokenOffset=0), dict(slot=0), dict(free=0), dict(poolIn=0),
                    dict(poolOut=0), dict(pageOffset=0), dict(stride=7), dict(stride=1 << 58), dict(table=64), dict(tokenOffset=128),
-                   dict(pageOffset=384), dict(slot=192), dict(poolOut=64), dict(slot=516), dict(held=66), dict(table=322)):
+                   dict(pageOffset=384), dict(slot=192), dict(poolOut=64), dict(poolOut=260), dict(poolOut=252), dict(slot=516), dict(held=66), dict(table=322)):
         assert rc(**change) == BAD, change
 
 
