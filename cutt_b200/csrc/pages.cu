@@ -138,6 +138,7 @@ constexpr int kMostBlocks = 16;
 __global__ void __launch_bounds__(1024)
 pages_build(const __grid_constant__ PagesBuild p, const int* poolIn, int* poolOut, int* tokenOffset, int* pageOffset, bool inPlace) {
   extern __shared__ int smem[];
+  begin_row_kernel();
   int* toks = smem;
   int* pags = smem + p.s.requests + 1;
   const Pool pool = read_pool(p, poolIn);
@@ -154,7 +155,7 @@ pages_build(const __grid_constant__ PagesBuild p, const int* poolIn, int* poolOu
 // Two kernels: prefix sums by one block, then the rest by many.
 __global__ void __launch_bounds__(1024)
 pages_scan(const __grid_constant__ PagesBuild p, const int* poolIn, int* poolOut, int* tokenOffset, int* pageOffset) {
-  cudaTriggerProgrammaticLaunchCompletion();
+  begin_row_kernel();
   const Pool pool = read_pool(p, poolIn);
   const uint2 sums = scan_requests(p, pool, tokenOffset, pageOffset, true, nullptr, nullptr);
   __syncthreads();          // every thread has read the pool, which may be updated in place
@@ -164,7 +165,7 @@ pages_scan(const __grid_constant__ PagesBuild p, const int* poolIn, int* poolOut
 constexpr int kExpandThreads = 256;
 
 __global__ void __launch_bounds__(kExpandThreads) pages_expand(const __grid_constant__ PagesBuild p) {
-  cudaGridDependencySynchronize();
+  begin_row_kernel();
   expand_requests(p, p.freeList ? clamp_pool(p.pool[1]) : 0, blockIdx.x, gridDim.x);
 }
 
@@ -189,6 +190,7 @@ struct PagedLaunch {
 template <int VB>
 __global__ void __launch_bounds__(kPagedThreads) paged_kernel(const __grid_constant__ PagedLaunch l) {
   typedef typename Raw<VB>::T R;
+  begin_row_kernel();
   const int q0 = blockIdx.x * l.p.perBlock;
   const unsigned char* src = l.m.src[blockIdx.y];
   unsigned char* dst = l.m.dst[blockIdx.y];
@@ -214,9 +216,7 @@ __global__ void __launch_bounds__(kPagedThreads) paged_kernel(const __grid_const
 template <int VB>
 cudaError_t paged_typed(const PagedLaunch& l, cudaStream_t stream) {
   const dim3 grid((unsigned)((l.p.s.tokens + l.p.perBlock - 1) / l.p.perBlock), l.m.tensors, 1);
-  paged_kernel<VB><<<grid, kPagedThreads, 0, stream>>>(l);
-  count_launch();
-  return cudaGetLastError();
+  return launch_row_kernel(paged_kernel<VB>, grid, kPagedThreads, 0, 0, stream, l);
 }
 
 }  // namespace
@@ -234,43 +234,13 @@ cudaError_t launch_pages_build(const PagesBuild& b, const int* poolIn, int* pool
     int blocks = 1;
     const int most = inPlace ? kMostBlocks : numSM;
     while (blocks * 2 <= most && b.s.maxTokens > blocks * kBlockTokens) blocks *= 2;
-    if (inPlace && blocks > 8) {
-      const cudaError_t e = cudaFuncSetAttribute(pages_build, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-      if (e != cudaSuccess) return e;
-    }
-    cudaLaunchAttribute cluster{};
-    cluster.id = cudaLaunchAttributeClusterDimension;
-    cluster.val.clusterDim.x = blocks;
-    cluster.val.clusterDim.y = 1;
-    cluster.val.clusterDim.z = 1;
-    cudaLaunchConfig_t c{};
-    c.gridDim = dim3(blocks);
-    c.blockDim = dim3(b.s.requests > 512 || b.s.maxTokens > 512 ? 1024 : 512);
-    c.dynamicSmemBytes = 8 * (b.s.requests + 1);
-    c.stream = stream;
-    c.attrs = &cluster;
-    c.numAttrs = inPlace ? 1 : 0;
-    const cudaError_t e = cudaLaunchKernelEx(&c, pages_build, b, poolIn, poolOut, tokenOffset, pageOffset, inPlace);
-    if (e == cudaSuccess) count_launch();
-    return e;
+    return launch_row_kernel(pages_build, dim3(blocks), b.s.requests > 512 || b.s.maxTokens > 512 ? 1024 : 512,
+                             8 * (b.s.requests + 1), inPlace ? blocks : 0, stream, b, poolIn, poolOut, tokenOffset, pageOffset, inPlace);
   }
-  pages_scan<<<1, 1024, 0, stream>>>(b, poolIn, poolOut, tokenOffset, pageOffset);
-  cudaError_t e = cudaGetLastError();
+  const cudaError_t e = launch_row_kernel(pages_scan, dim3(1), 1024, 0, 0, stream, b, poolIn, poolOut, tokenOffset, pageOffset);
   if (e != cudaSuccess) return e;
-  count_launch();
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t c{};
-  const int want = (b.s.maxTokens + kExpandThreads - 1) / kExpandThreads;
-  c.gridDim = dim3(want < numSM * 8 ? want : numSM * 8);
-  c.blockDim = dim3(kExpandThreads);
-  c.stream = stream;
-  c.attrs = &attr;
-  c.numAttrs = 1;
-  e = cudaLaunchKernelEx(&c, pages_expand, b);
-  if (e == cudaSuccess) count_launch();
-  return e;
+  const int want = (b.s.maxTokens + kExpandThreads - 1) / kExpandThreads, most = numSM * 8;
+  return launch_row_kernel(pages_expand, dim3(want < 1 ? 1 : want < most ? want : most), kExpandThreads, 0, 0, stream, b);
 }
 
 cudaError_t launch_paged(const PagedShape& s, const PagedMove& m, cudaStream_t stream) {

@@ -2,9 +2,55 @@
 #pragma once
 #include <cuda_runtime.h>
 
+#include "kernels.h"
+
 #include "rows_plan.h"
 
 namespace cuttb {
+
+// Launch of a row operator's kernel.  The kernels of a step follow one another in microseconds, so each
+// is launched while the one before it still runs (programmatic dependent launch) and waits, as its first
+// statement, for that one's end: begin_row_kernel.  It lets the next kernel start in turn only then, so
+// whatever precedes this kernel in the stream is done before the next one begins, and a kernel may read
+// this one's INPUTS before it waits itself.  Inputs are read with coherent loads (no __restrict__): a line
+// may have come into the cache before the kernel that writes it ended.
+// `cluster`: blocks of a cluster, 0 for none.
+template <typename... P, typename... A>
+cudaError_t launch_row_kernel(void (*kernel)(P...), dim3 grid, int threads, size_t smem, int cluster, cudaStream_t stream, A... args) {
+  if (smem > 40 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+  }
+  if (cluster > 8) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return e;
+  }
+  cudaLaunchAttribute attr[2] = {};
+  cudaLaunchConfig_t c{};
+  c.gridDim = grid;
+  c.blockDim = dim3(threads);
+  c.dynamicSmemBytes = smem;
+  c.stream = stream;
+  c.attrs = attr;
+  attr[c.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[c.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+  if (cluster > 1) {
+    attr[c.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attr[c.numAttrs].val.clusterDim.x = cluster;
+    attr[c.numAttrs].val.clusterDim.y = 1;
+    attr[c.numAttrs++].val.clusterDim.z = 1;
+  }
+  const cudaError_t e = cudaLaunchKernelEx(&c, kernel, P(args)...);
+  if (e == cudaSuccess) count_launch();
+  return e;
+}
+
+#ifdef __CUDACC__
+__device__ __forceinline__ void begin_row_kernel() {
+  cudaGridDependencySynchronize();
+  cudaTriggerProgrammaticLaunchCompletion();
+}
+#endif
 
 cudaError_t launch_rows_sort(const RowsShape& s, const void* expertOf, int indexBytes, int* count, int* offset,
                              int* rowOf, int* slotOf, int numSM, cudaStream_t stream);

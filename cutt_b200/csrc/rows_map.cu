@@ -201,9 +201,10 @@ constexpr int kMostBlocks = 16;
 // distributed shared memory, so there is one launch and no workspace.
 template <typename I>
 __global__ void __launch_bounds__(1024)
-sort_cluster(RowsShape s, const I* __restrict__ ids, int slots, int* count, int* offset, int* rowOf, int* slotOf) {
+sort_cluster(RowsShape s, const I* ids, int slots, int* count, int* offset, int* rowOf, int* slotOf) {
   extern __shared__ int smem[];
   __shared__ int2 scratch[32];
+  begin_row_kernel();
   cg::cluster_group cluster = cg::this_cluster();
   const int blocks = gridDim.x, me = blockIdx.x, E = s.experts;
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, nw = blockDim.x >> 5;
@@ -271,9 +272,9 @@ __device__ __forceinline__ void chunk_range(int n, int chunk, int chunks, int b,
 
 template <typename I>
 __global__ void __launch_bounds__(kChunkThreads)
-sort_count(RowsShape s, const I* __restrict__ ids, int* rowOf, int chunk, int chunks) {
+sort_count(RowsShape s, const I* ids, int* rowOf, int chunk, int chunks) {
   extern __shared__ int hist[];
-  cudaTriggerProgrammaticLaunchCompletion();
+  begin_row_kernel();
   const int w = threadIdx.x >> 5, nw = blockDim.x >> 5;
   int lo, hi;
   chunk_range(s.tokens * s.choices, chunk, chunks, blockIdx.x, lo, hi);
@@ -309,6 +310,7 @@ sort_starts(RowsShape s, int* count, int* offset, int* rowOf, int chunk, int chu
   __shared__ int start[kMostPart];
   __shared__ int2 scratch[32];
   cg::cluster_group cluster = cg::this_cluster();
+  // the last kernel may start its ranks: the inputs are complete, sort_count saw to that
   cudaTriggerProgrammaticLaunchCompletion();
   cudaGridDependencySynchronize();
   const int E = s.experts, own = (E + kStartBlocks - 1) / kStartBlocks;
@@ -371,7 +373,7 @@ sort_starts(RowsShape s, int* count, int* offset, int* rowOf, int chunk, int chu
 
 template <typename I>
 __global__ void __launch_bounds__(1024)
-sort_rows(RowsShape s, const I* __restrict__ ids, const int* count, const int* offset, int* rowOf, int* slotOf, int chunk,
+sort_rows(RowsShape s, const I* ids, const int* count, const int* offset, int* rowOf, int* slotOf, int chunk,
           int chunks, int slots) {
   extern __shared__ int smem[];
   __shared__ int2 scratch[32];
@@ -380,7 +382,7 @@ sort_rows(RowsShape s, const I* __restrict__ ids, const int* count, const int* o
   chunk_range(s.tokens * s.choices, chunk, chunks, blockIdx.x, lo, hi);
   const Ranked r = carve(smem, slots, nw, E);
   rank_block(s, ids, lo, hi, r);         // does not need the kernels before this one
-  cudaGridDependencySynchronize();
+  begin_row_kernel();
   int carry = 0;
   for (int e0 = 0; e0 < E; e0 += blockDim.x) {
     const int e = e0 + threadIdx.x;
@@ -395,38 +397,6 @@ sort_rows(RowsShape s, const I* __restrict__ ids, const int* count, const int* o
   __syncthreads();
   write_block(s, lo, hi, r, carry, rowOf, slotOf);
   fill_gaps(E, s.capacity, count, offset, slotOf, blockIdx.x, gridDim.x);
-}
-
-template <typename... P, typename... A>
-cudaError_t launch(void (*kernel)(P...), int grid, int threads, int words, int cluster, bool early, cudaStream_t stream, A... args) {
-  if (words > 10 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, words * 4);
-    if (e != cudaSuccess) return e;
-  }
-  if (cluster > 8) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-    if (e != cudaSuccess) return e;
-  }
-  cudaLaunchAttribute attr[2] = {};
-  cudaLaunchConfig_t c{};
-  c.gridDim = dim3(grid);
-  c.blockDim = dim3(threads);
-  c.dynamicSmemBytes = words * 4;
-  c.stream = stream;
-  c.attrs = attr;
-  if (early) {
-    attr[c.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[c.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
-  }
-  if (cluster > 1) {
-    attr[c.numAttrs].id = cudaLaunchAttributeClusterDimension;
-    attr[c.numAttrs].val.clusterDim.x = cluster;
-    attr[c.numAttrs].val.clusterDim.y = 1;
-    attr[c.numAttrs++].val.clusterDim.z = 1;
-  }
-  const cudaError_t e = cudaLaunchKernelEx(&c, kernel, P(args)...);
-  if (e == cudaSuccess) count_launch();
-  return e;
 }
 
 // Up to this many slots a cluster, above three kernels.  Measured, 128 experts: 32768 slots 6.2
@@ -461,8 +431,8 @@ cudaError_t sort_typed(const RowsShape& s, const I* ids, int* count, int* offset
     const int slots = ((n + blocks - 1) / blocks + 31) & ~31;
     int warps = warps_for(slots, E, kBlockWarps);
     while (warps > 4 && warps * 32 > slots) warps >>= 1;
-    return launch(sort_cluster<I>, blocks, warps * 32, ranked_words(slots, warps, E) + 3 * E, blocks, false, stream, s, ids, slots,
-                  count, offset, rowOf, slotOf);
+    return launch_row_kernel(sort_cluster<I>, dim3(blocks), warps * 32, (ranked_words(slots, warps, E) + 3 * E) * 4, blocks, stream, s,
+                             ids, slots, count, offset, rowOf, slotOf);
   }
   // one chunk for an SM: more of them are more rows of the table of counts (524288 slots: 148 chunks
   // 15.6 us, 296 chunks 18.5)
@@ -473,13 +443,13 @@ cudaError_t sort_typed(const RowsShape& s, const I* ids, int* count, int* offset
   int chunks = n / chunk;
   if (chunks == 0 || n - chunks * chunk >= E) chunks++;    // else the last one takes the rest
   const int slots = (chunk + E + 31) & ~31;
-  cudaError_t e = launch(sort_count<I>, chunks, kChunkThreads, E, 0, false, stream, s, ids, rowOf, chunk, chunks);
+  cudaError_t e = launch_row_kernel(sort_count<I>, dim3(chunks), kChunkThreads, E * 4, 0, stream, s, ids, rowOf, chunk, chunks);
   if (e != cudaSuccess) return e;
-  e = launch(sort_starts, kStartBlocks, kChunkThreads, 0, 0, true, stream, s, count, offset, rowOf, chunk, chunks);
+  e = launch_row_kernel(sort_starts, dim3(kStartBlocks), kChunkThreads, 0, 0, stream, s, count, offset, rowOf, chunk, chunks);
   if (e != cudaSuccess) return e;
   const int warps = warps_for(slots, E, kBlockWarps);
-  return launch(sort_rows<I>, chunks, warps * 32, ranked_words(slots, warps, E), 0, true, stream, s, ids, count, offset,
-                rowOf, slotOf, chunk, chunks, slots);
+  return launch_row_kernel(sort_rows<I>, dim3(chunks), warps * 32, ranked_words(slots, warps, E) * 4, 0, stream, s, ids, count,
+                           offset, rowOf, slotOf, chunk, chunks, slots);
 }
 
 }  // namespace

@@ -212,6 +212,7 @@ template <typename T, bool ANY, int KU, int THREADS, bool WEIGHT, bool DOT>
 __global__ void __launch_bounds__(THREADS, scatter_warps(ANY, DOT) * 32 / THREADS)
 scatter_kernel(const __grid_constant__ RowsMove m, int padBlocks) {
   __shared__ float part[THREADS / 32][KU];
+  begin_row_kernel();
   const int bytes = m.width * (int)sizeof(T);
   const int vecs = bytes / 16 + (ANY ? 2 : 0);
   const int share = (vecs + gridDim.y - 1) / gridDim.y;
@@ -307,6 +308,7 @@ template <typename T, bool ANY, int KU, int THREADS, bool DOT>
 __global__ void __launch_bounds__(THREADS, gather_warps(KU) * 32 / THREADS)
 gather_kernel(const __grid_constant__ RowsMove m) {
   __shared__ float part[THREADS / 32][KU];
+  begin_row_kernel();
   constexpr int N = Piece<T>::N;
   // pieces that the block takes at once: with ANY the last lane of every warp only lends its bytes
   constexpr int STEP = ANY ? THREADS / 32 * 31 : THREADS;
@@ -446,24 +448,21 @@ dim3 token_grid(const RowsMove& m, int vecs, int threads, bool few) {
 }
 
 template <typename T, bool ANY, int KU, int THREADS>
-void run_scatter_dot(const RowsMove& m, dim3 grid, int pad, cudaStream_t stream) {
-  if (m.weight) scatter_kernel<T, ANY, KU, THREADS, true, true><<<grid, THREADS, 0, stream>>>(m, pad);
-  else scatter_kernel<T, ANY, KU, THREADS, false, true><<<grid, THREADS, 0, stream>>>(m, pad);
+cudaError_t run_scatter_dot(const RowsMove& m, dim3 grid, int pad, cudaStream_t stream) {
+  if (m.weight) return launch_row_kernel(scatter_kernel<T, ANY, KU, THREADS, true, true>, grid, THREADS, 0, 0, stream, m, pad);
+  return launch_row_kernel(scatter_kernel<T, ANY, KU, THREADS, false, true>, grid, THREADS, 0, 0, stream, m, pad);
 }
 
 template <typename T, bool ANY, int KU, int THREADS>
-void run_scatter(const RowsMove& m, dim3 grid, int pad, cudaStream_t stream) {
+cudaError_t run_scatter(const RowsMove& m, dim3 grid, int pad, cudaStream_t stream) {
   if constexpr (sizeof(T) > 1 && THREADS <= 256) {
-    if (m.weight) {
-      scatter_kernel<T, ANY, KU, THREADS, true, false><<<grid, THREADS, 0, stream>>>(m, pad);
-      return;
-    }
+    if (m.weight) return launch_row_kernel(scatter_kernel<T, ANY, KU, THREADS, true, false>, grid, THREADS, 0, 0, stream, m, pad);
   }
-  scatter_kernel<T, ANY, KU, THREADS, false, false><<<grid, THREADS, 0, stream>>>(m, pad);
+  return launch_row_kernel(scatter_kernel<T, ANY, KU, THREADS, false, false>, grid, THREADS, 0, 0, stream, m, pad);
 }
 
 template <typename T, bool ANY, int KU>
-void scatter(const RowsMove& m, int pad, int numSM, cudaStream_t stream) {
+cudaError_t scatter(const RowsMove& m, int pad, int numSM, cudaStream_t stream) {
   const int vecs = m.width * (int)sizeof(T) / 16 + (ANY ? 2 : 0);
   const bool few = m.tokens < numSM * kFewTokens;
   // (rows at any address: four at a time, see move_rows)
@@ -472,50 +471,50 @@ void scatter(const RowsMove& m, int pad, int numSM, cudaStream_t stream) {
       const int threads = sum_threads(m, vecs, numSM);
       dim3 g = token_grid(m, vecs, threads, few);
       g.x += pad;
-      if (threads == 256) run_scatter_dot<T, ANY, KU, 256>(m, g, pad, stream);
-      else if (threads == 128) run_scatter_dot<T, ANY, KU, 128>(m, g, pad, stream);
-      else run_scatter_dot<T, ANY, KU, 64>(m, g, pad, stream);
-      return;
+      if (threads == 256) return run_scatter_dot<T, ANY, KU, 256>(m, g, pad, stream);
+      if (threads == 128) return run_scatter_dot<T, ANY, KU, 128>(m, g, pad, stream);
+      return run_scatter_dot<T, ANY, KU, 64>(m, g, pad, stream);
     }
   }
   const int threads = few ? 128 : scatter_threads((long long)m.choices * vecs, m.weight != nullptr);
   dim3 g = token_grid(m, vecs, threads, few);
   g.x += pad;
-  if (threads == 512) run_scatter<T, ANY, KU, 512>(m, g, pad, stream);
-  else if (threads == 256) run_scatter<T, ANY, KU, 256>(m, g, pad, stream);
-  else if (threads == 128) run_scatter<T, ANY, KU, 128>(m, g, pad, stream);
-  else run_scatter<T, ANY, KU, 64>(m, g, pad, stream);
+  if (threads == 512) return run_scatter<T, ANY, KU, 512>(m, g, pad, stream);
+  if (threads == 256) return run_scatter<T, ANY, KU, 256>(m, g, pad, stream);
+  if (threads == 128) return run_scatter<T, ANY, KU, 128>(m, g, pad, stream);
+  return run_scatter<T, ANY, KU, 64>(m, g, pad, stream);
 }
 
 template <typename T, bool ANY, int KU>
-void gather(const RowsMove& m, int numSM, cudaStream_t stream) {
+cudaError_t gather(const RowsMove& m, int numSM, cudaStream_t stream) {
   const int vecs = m.width * (int)sizeof(T) / 16 + (ANY ? 2 : 0);
   const bool few = m.tokens < numSM * kFewTokens;
   if (m.dweight) {
     const int threads = few ? sum_threads(m, vecs, numSM) : vecs >= 512 ? 128 : 64;
     const dim3 g = token_grid(m, vecs, threads, few);
-    if (threads == 256) gather_kernel<T, ANY, KU, 256, true><<<g, 256, 0, stream>>>(m);
-    else if (threads == 128) gather_kernel<T, ANY, KU, 128, true><<<g, 128, 0, stream>>>(m);
-    else gather_kernel<T, ANY, KU, 64, true><<<g, 64, 0, stream>>>(m);
-    return;
+    if (threads == 256) return launch_row_kernel(gather_kernel<T, ANY, KU, 256, true>, g, 256, 0, 0, stream, m);
+    if (threads == 128) return launch_row_kernel(gather_kernel<T, ANY, KU, 128, true>, g, 128, 0, 0, stream, m);
+    return launch_row_kernel(gather_kernel<T, ANY, KU, 64, true>, g, 64, 0, 0, stream, m);
   }
   const int threads = few || vecs >= 512 ? 128 : 64;
   const dim3 g = token_grid(m, vecs, threads, few);
-  if (threads == 128) gather_kernel<T, ANY, KU, 128, false><<<g, 128, 0, stream>>>(m);
-  else gather_kernel<T, ANY, KU, 64, false><<<g, 64, 0, stream>>>(m);
+  if (threads == 128) return launch_row_kernel(gather_kernel<T, ANY, KU, 128, false>, g, 128, 0, 0, stream, m);
+  return launch_row_kernel(gather_kernel<T, ANY, KU, 64, false>, g, 64, 0, 0, stream, m);
 }
 
 template <typename T, bool ANY>
-void move_rows(const RowsMove& m, bool rowsOut, int pad, int numSM, cudaStream_t stream) {
+cudaError_t move_rows(const RowsMove& m, bool rowsOut, int pad, int numSM, cudaStream_t stream) {
   if (rowsOut) {
     // Four or eight of a token's rows at a time.  At any address and with the weights' gradient eight leave
     // too few registers for enough warps: 16384 tokens, 8 rows of 2001 bf16, 471 us, with four 361.
-    if (m.choices <= 4 || (ANY && m.dweight)) scatter<T, ANY, 4>(m, pad, numSM, stream);
-    else scatter<T, ANY, 8>(m, pad, numSM, stream);
-  } else if constexpr (sizeof(T) > 1) {
-    if (m.choices <= 4) gather<T, ANY, 4>(m, numSM, stream);
-    else gather<T, ANY, 8>(m, numSM, stream);
+    if (m.choices <= 4 || (ANY && m.dweight)) return scatter<T, ANY, 4>(m, pad, numSM, stream);
+    return scatter<T, ANY, 8>(m, pad, numSM, stream);
   }
+  if constexpr (sizeof(T) > 1) {
+    if (m.choices <= 4) return gather<T, ANY, 4>(m, numSM, stream);
+    return gather<T, ANY, 8>(m, numSM, stream);
+  }
+  return cudaErrorInvalidValue;          // bytes are not summed: check_rows_move
 }
 
 template <typename T>
@@ -524,10 +523,7 @@ cudaError_t move_typed(const RowsMove& m, bool rowsOut, int pad, int numSM, cuda
   unsigned long long bits = (uintptr_t)m.token | (uintptr_t)m.row | (uintptr_t)m.other | (unsigned long long)m.tokenStride |
                             (unsigned long long)m.rowStride | (unsigned long long)(m.width * (long long)sizeof(T));
   if (m.other) bits |= (unsigned long long)m.otherStride;
-  if (bits % 16) move_rows<T, true>(m, rowsOut, pad, numSM, stream);
-  else move_rows<T, false>(m, rowsOut, pad, numSM, stream);
-  count_launch();
-  return cudaGetLastError();
+  return bits % 16 ? move_rows<T, true>(m, rowsOut, pad, numSM, stream) : move_rows<T, false>(m, rowsOut, pad, numSM, stream);
 }
 
 cudaError_t move(const RowsMove& m, bool rowsOut, int pad, int numSM, cudaStream_t stream) {
