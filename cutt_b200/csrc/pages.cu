@@ -3,7 +3,6 @@
 #include <cooperative_groups.h>
 #include <stdint.h>
 
-#include "kernels.h"
 #include "rows.h"
 
 namespace cuttb {
@@ -123,8 +122,8 @@ __device__ __forceinline__ void expand_requests(const PagesBuild& p, int limit, 
   }
   if (!p.freeList) return;
   const int end = p.pageOffset[p.s.requests];
-  for (int f = p.pageOffset[0] + at; f < end; f += stride)
-    take_page(p, last_at_or_before(p.pageOffset, p.s.requests + 1, f), f, limit);
+  for (long long f = (long long)p.pageOffset[0] + at; f < end; f += stride)      // end may be close to 2^31
+    take_page(p, last_at_or_before(p.pageOffset, p.s.requests + 1, (int)f), (int)f, limit);
 }
 
 // One kernel.  Every block makes all prefix sums for itself, in shared memory: a few kilobytes of

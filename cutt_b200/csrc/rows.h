@@ -3,7 +3,6 @@
 #include <cuda_runtime.h>
 
 #include "kernels.h"
-
 #include "rows_plan.h"
 
 namespace cuttb {

@@ -69,7 +69,11 @@ int check_device(const Plan& p) {
   return dev == p.device ? CUTT_SUCCESS : CUTT_INVALID_DEVICE;
 }
 
-int result(cudaError_t e) { return e == cudaSuccess ? CUTT_SUCCESS : CUTT_INTERNAL_ERROR; }
+int result(cudaError_t e) {
+  if (e == cudaSuccess) return CUTT_SUCCESS;
+  cudaGetLastError();        // reported here, not by the caller's next CUDA call
+  return CUTT_INTERNAL_ERROR;
+}
 
 int move_rows(unsigned int handle, const RowsMoveArgs& a) {
   const std::shared_ptr<const Plan> p = find_plan(handle, kRows);

@@ -12,7 +12,6 @@
 #include <cooperative_groups.h>
 #include <stdint.h>
 
-#include "kernels.h"
 #include "rows.h"
 
 namespace cuttb {
@@ -401,7 +400,7 @@ sort_rows(RowsShape s, const I* ids, const int* count, const int* offset, int* r
 
 // Up to this many slots a cluster, above three kernels.  Measured, 128 experts: 32768 slots 6.2
 // against 8.1 us, 65536 slots 7.5 against 8.3 us, and one launch against three; 524288 slots of 256
-// experts take 14 us in three kernels.
+// experts take 13 us in three kernels.
 constexpr int kClusterSlots = 65536;
 // A block takes this many slots where one is enough, else half of them, and more once the cluster is
 // full: 512 slots 4.4 us in one block, 4.2 in two; 288 slots 3.8 and 4.5; 1024 slots 4.6 in four, 5.2

@@ -15,7 +15,6 @@
 #include <cuda_fp16.h>
 #include <stdint.h>
 
-#include "kernels.h"
 #include "rows.h"
 
 namespace cuttb {

@@ -98,7 +98,7 @@ int cutt_pages_plan(unsigned int* handle, int requests, int pageSize, int tableW
  *   slot[maxTokens]            of new token i of request b, at tokenOffset[b] + i: page * pageSize +
  *                              place in the page, from the table; -1 where there is no page and
  *                              behind the last token.  Tokens at or beyond maxTokens get no entry.
- *   pool                       {next free entry, entries} of freeList; poolOut = {min(pageOffset[
+ *   pool                       {next free entry, entries} of freeList (at most 2^30); poolOut = {min(pageOffset[
  *                              requests], max(pool[0], pool[1])), pool[1]} and may be the same address.
  * pageOffset[requests] > pool[1] says that pages ran short, and by how many.
  * With freeList NULL (then poolIn, poolOut and pageOffset are NULL too) no page is taken and the

@@ -121,6 +121,33 @@ def test_long_build_captured_with_the_pool_in_place(native):
         held = [x + y for x, y in zip(held, added)]
 
 
+@pytest.mark.parametrize("b,n,steps", [(6, 1, 300), (40, 300, 25), (3, 9000, 4)])
+def test_steps_without_a_pause(native, b, n, steps):
+    """Tables, stores and loads one behind the other with nothing between them; errors counted on the device."""
+    import torch
+    page, heads, size = 8, 2, 16
+    m = b * n
+    width = -(-n * steps // page) + 1
+    pages = b * width + 1
+    c = Build(native, [0] * b, [n] * b, page, width, list(range(1, pages)), [0, pages - 1], m)
+    rows = native.PagedRows(m, heads, size, 4, pages, page, heads * page * size, size, page * size,
+                            stream=torch.cuda.current_stream().cuda_stream)
+    cache, src, back = torch.zeros(pages, heads, page, size, device="cuda"), torch.randn(m, heads, size, device="cuda"), torch.zeros(m, heads, size, device="cuda")
+    wrong = torch.zeros(1, dtype=torch.int64, device="cuda")
+    for i in range(steps):
+        src.add_(1.0)
+        c.build()
+        rows.store(src.data_ptr(), 0, c.slot.data_ptr(), cache.data_ptr(), 0)
+        rows.load(cache.data_ptr(), 0, c.slot.data_ptr(), back.data_ptr(), 0)
+        c.held.add_(n)
+        wrong += (back != src).any() + (c.slot[:m] < 0).any() + (c.slot[:m].sort().values.diff() == 0).any()
+    assert wrong.item() == 0
+    taken = b * -(-n * steps // page)
+    assert c.pool.tolist() == [taken, pages - 1]
+    used = c.table[:, :-(-n * steps // page)]
+    assert used.unique().numel() == taken
+
+
 def test_build_of_empty_and_odd_lengths(native):
     for held, added in (([0, 0, 0], [0, 0, 0]), ([0], [0]), ([-5, 7, -1], [3, -9, 0]), ([100, 32, 31], [5, 1, 2])):
         c = Build(native, held, added, 8, 4, list(range(50, 70)), [2, 20], 9)

@@ -517,6 +517,32 @@ def test_layer_captured_and_replayed_with_new_routing(native):
             assert torch.equal(getattr(captured, name), getattr(eager, name)), name
 
 
+@pytest.mark.parametrize("t,e,steps", [(40, 16, 400), (3000, 64, 200), (20000, 48, 60)])
+def test_steps_without_a_pause(native, t, e, steps):
+    """Kernels that start while the one before still runs: buffers that change from step to step, nothing
+    between the calls, errors counted on the device."""
+    import torch
+    k, h = 4, 128
+    r = Run(native, routing(t, k, e, 1), h, "f32", e, align=4)
+    g = torch.Generator().manual_seed(3)
+    base, x = r.ids.clone(), torch.randn(t, h, generator=g).cuda()
+    rows, out = torch.zeros(r.r, h, device="cuda"), torch.zeros(t, h, device="cuda")
+    dx, dy = torch.zeros(t, h, device="cuda"), torch.zeros(r.r, h, device="cuda")
+    wrong = torch.zeros(1, dtype=torch.int64, device="cuda")
+    slots = torch.arange(t * k, device="cuda").view(t, k)
+    for i in range(steps):
+        r.ids.copy_((base + i) % e)
+        x.add_(1.0)
+        r.sort()
+        r.plan.dispatch(x.data_ptr(), *r.maps(), rows.data_ptr())
+        r.plan.combine(rows.data_ptr(), r.row_of.data_ptr(), out.data_ptr())
+        r.plan.combine_grad(out.data_ptr(), *r.maps(), dy.data_ptr())
+        r.plan.dispatch_grad(dy.data_ptr(), r.row_of.data_ptr(), dx.data_ptr())
+        wrong += (out != 4 * x).any() + (dx != 16 * x).any() + (r.slot_of[r.row_of.long()] != slots).any()
+        wrong += (r.count != torch.bincount(r.ids.view(-1).long(), minlength=e)).any()
+    assert wrong.item() == 0          # sums of 4 and 16 equal numbers are exact
+
+
 def test_two_plans_on_two_streams_at_once(native):
     import torch
     sets = []
