@@ -543,6 +543,88 @@ def test_steps_without_a_pause(native, t, e, steps):
     assert wrong.item() == 0          # sums of 4 and 16 equal numbers are exact
 
 
+def test_capture_behind_copies_and_other_streams(native):
+    """Graph nodes before the operators that are not kernels (copies, a fill), and a join with another stream."""
+    import torch
+    side, other = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        r = Run(native, routing(500, 4, 30, 1), 256, "bf16", 30, align=8)
+        r.sort()
+    new_ids, new_x = r.ids.clone(), torch.zeros(500, 256, dtype=torch.bfloat16, device="cuda")
+    x, rows = torch.zeros_like(new_x), torch.zeros(r.r, 256, dtype=torch.bfloat16, device="cuda")
+    out = torch.zeros_like(x)
+    host = torch.zeros(500, 256, dtype=torch.bfloat16).pin_memory()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        other.wait_stream(side)
+        with torch.cuda.stream(other):
+            x.copy_(new_x)
+        r.ids.copy_(new_ids)                      # a copy node
+        r.sort()
+        rows.zero_()                              # a fill node
+        side.wait_stream(other)                   # two dependencies
+        r.plan.dispatch(x.data_ptr(), *r.maps(), rows.data_ptr())
+        r.plan.combine(rows.data_ptr(), r.row_of.data_ptr(), out.data_ptr())
+        host.copy_(out, non_blocking=True)
+    g = torch.Generator().manual_seed(2)
+    for seed in (4, 5, 6):
+        ids = routing(500, 4, 30, seed)
+        new_ids.copy_(ids)
+        new_x.copy_(torch.randn(500, 256, generator=g))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        r.want = plain_map(ids.reshape(-1).tolist(), 0, 30, 8, r.r)
+        r.check_map()
+        assert torch.equal(host, (4 * new_x.float()).bfloat16().cpu())
+        assert (rows[r.want[1][-1]:] == 0).all()
+
+
+def test_one_plan_from_several_threads(native):
+    import threading
+    import torch
+    r = Run(native, routing(200, 4, 12, 1), 512, "f32", 12)
+    r.sort()
+    x, rows = torch.randn(200, 512, device="cuda"), torch.zeros(r.r, 512, device="cuda")
+    r.plan.dispatch(x.data_ptr(), *r.maps(), rows.data_ptr())
+    outs = [torch.zeros(200, 512, device="cuda") for _ in range(4)]
+    failed = []
+
+    def work(out):
+        try:
+            torch.cuda.set_device(0)
+            for _ in range(200):
+                r.plan.combine(rows.data_ptr(), r.row_of.data_ptr(), out.data_ptr())
+                p = native.RowPlan(3, 1, 2, 8, native.CUTT_ROWS_F32)
+                p.destroy()
+        except Exception as e:
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(o,)) for o in outs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not failed
+    for out in outs:
+        assert torch.equal(out, 4 * x)
+
+
+def test_calls_on_another_device_are_refused(native):
+    import torch
+    if torch.cuda.device_count() < 2:
+        pytest.skip("needs two GPUs")
+    r = Run(native, routing(20, 2, 4, 1), 32, "f32", 4)
+    with torch.cuda.device(1):
+        with pytest.raises(native.CuttError) as e:
+            r.sort()
+    assert e.value.code == native.CUTT_INVALID_DEVICE
+    r.sort()
+    r.check_map()
+
+
 def test_two_plans_on_two_streams_at_once(native):
     import torch
     sets = []
