@@ -196,9 +196,10 @@ __device__ __forceinline__ bool near_rows(const RowsMove& m, const int (&row)[KU
 // pieces of many rows needs registers, the others do better with more warps.  Measured, us: rows out
 // with the weights' gradient (16384 tokens, half of 8 slots dropped, 4 KB) 24 warps 110, 32 warps 124;
 // 16384 tokens to 8 rows of 2001 bf16 with 32, 48, 64 warps 119, 126, 132; sums of 8 rows of 4 KB, half
-// dropped, 24, 28, 32 warps 60, 57, 59; sums of 4 rows of 5 KB 32, 40, 48 warps 36.2, 35.2, 35.5.
+// dropped, 24, 28, 32 warps 60, 57, 59; sums of 4 rows of 5 KB 32, 40, 48 warps 36.2, 35.2, 35.5; sums of 10
+// rows of 4 KB with the weights' gradient 16, 20, 24 warps 171, 110, 139.
 constexpr int scatter_warps(bool, bool dot) { return dot ? 24 : 32; }
-constexpr int gather_warps(int ku) { return ku > 4 ? 28 : 40; }
+constexpr int gather_warps(int ku) { return ku > 8 ? 20 : ku > 4 ? 28 : 40; }
 
 // ANY: rows at any address; the pieces of a row are then cut at the 16-byte boundaries of the row
 // that is written, so its first and last pieces may be partial.  The token's words are cut at its
@@ -309,6 +310,7 @@ gather_kernel(const __grid_constant__ RowsMove m) {
   __shared__ float part[THREADS / 32][KU];
   begin_row_kernel();
   constexpr int N = Piece<T>::N;
+  constexpr int H = KU < 8 ? KU : 8;       // rows whose pieces are loaded at once
   // pieces that the block takes at once: with ANY the last lane of every warp only lends its bytes
   constexpr int STEP = ANY ? THREADS / 32 * 31 : THREADS;
   const int bytes = m.width * (int)sizeof(T);
@@ -327,49 +329,64 @@ gather_kernel(const __grid_constant__ RowsMove m) {
   // Up to KU choices: one walk over the row does everything.  More: the weights' gradient takes a
   // walk for each group of KU slots, then one walk sums over all groups in registers.
   const bool one = m.choices <= KU;
-  int row[KU];
-  float w[KU];
+  // KU of 16: the rows of the eight that are at work only, read again for every piece (they stay in L1), so
+  // that registers are left for enough warps.
+  constexpr bool AGAIN = KU > H;
+  int row[H];
+  float w[H];
   bool near = false;
   if (one || DOT) {
     for (int j0 = 0; j0 < m.choices; j0 += KU) {
       float dot[KU];
-      load_slots<KU>(m, s0, j0, row, w);
-      if (ANY) near = near_rows<KU>(m, row, m.rowStride);
+      if (!AGAIN) {
+        load_slots<H>(m, s0, j0, row, w);
+        if (ANY) near = near_rows<H>(m, row, m.rowStride);
+      }
 #pragma unroll
       for (int j = 0; j < KU; j++) dot[j] = 0.f;
       for (int v = v0 + first; ANY ? __any_sync(0xffffffffu, v < v1) : v < v1; v += STEP) {
         const int lo = v * 16 - mis;
-        Piece<T> b[KU], a;
+        const bool idle = v >= v1 || (ANY && (lender || lo >= bytes));      // (without ANY: never)
+        Piece<T> b[H], a;
         float sum[N];
 #pragma unroll
         for (int i = 0; i < N; i++) sum[i] = 0.f;
-#pragma unroll
-        for (int j = 0; j < KU; j++) {
-          if (row[j] < 0) continue;
-          const unsigned char* y = m.row + (long long)row[j] * m.rowStride;
-          b[j].raw = ANY ? load_word<T>(y, lo, bytes, near) : load_16(y + lo);
-        }
         if (DOT) a.raw = ANY ? load_word<T>(x, lo, bytes, nearX) : load_16(x + lo);
-        if (ANY && DOT) a.raw = join_words(a.raw, x, lo);
-        if (ANY) {
 #pragma unroll
-          for (int j = 0; j < KU; j++)
-            if (row[j] >= 0) b[j].raw = join_words(b[j].raw, m.row + (long long)row[j] * m.rowStride, lo);
-          if (lender || v >= v1 || lo >= bytes) continue;
-        }
-        if (ANY && DOT) clear_outside(a, lo, bytes);
+        for (int h = 0; h < KU; h += H) {
+          if (AGAIN) {
+            load_slots<H>(m, s0, j0 + h, row, w);
+            if (ANY) near = near_rows<H>(m, row, m.rowStride);
+          }
 #pragma unroll
-        for (int j = 0; j < KU; j++) {
-          if (row[j] < 0) continue;
-          if (ANY && DOT) clear_outside(b[j], lo, bytes);
+          for (int j = 0; j < H; j++) {
+            if (row[j] < 0) continue;
+            const unsigned char* y = m.row + (long long)row[j] * m.rowStride;
+            b[j].raw = ANY ? load_word<T>(y, lo, bytes, near) : load_16(y + lo);
+          }
+          if (ANY) {
 #pragma unroll
-          for (int i = 0; i < N; i++) {
-            const float f = to_f(b[j].e[i]);
-            sum[i] = fmaf(w[j], f, sum[i]);
-            if (DOT) dot[j] = fmaf(f, to_f(a.e[i]), dot[j]);
+            for (int j = 0; j < H; j++)
+              if (row[j] >= 0) b[j].raw = join_words(b[j].raw, m.row + (long long)row[j] * m.rowStride, lo);
+            if (DOT && h == 0) {
+              a.raw = join_words(a.raw, x, lo);
+              clear_outside(a, lo, bytes);
+            }
+            if (idle) continue;
+          }
+#pragma unroll
+          for (int j = 0; j < H; j++) {
+            if (row[j] < 0) continue;
+            if (ANY && DOT) clear_outside(b[j], lo, bytes);
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+              const float f = to_f(b[j].e[i]);
+              sum[i] = fmaf(w[j], f, sum[i]);
+              if (DOT) dot[h + j] = fmaf(f, to_f(a.e[i]), dot[h + j]);
+            }
           }
         }
-        if (one) {
+        if (one && !idle) {
           Piece<T> r;
 #pragma unroll
           for (int i = 0; i < N; i++) r.e[i] = from_f<T>(sum[i]);
@@ -386,18 +403,18 @@ gather_kernel(const __grid_constant__ RowsMove m) {
     float sum[N];
 #pragma unroll
     for (int i = 0; i < N; i++) sum[i] = 0.f;
-    for (int j0 = 0; j0 < m.choices; j0 += KU) {
-      Piece<T> b[KU];
-      load_slots<KU>(m, s0, j0, row, w);
-      if (ANY) near = near_rows<KU>(m, row, m.rowStride);
+    for (int j0 = 0; j0 < m.choices; j0 += H) {
+      Piece<T> b[H];
+      load_slots<H>(m, s0, j0, row, w);
+      if (ANY) near = near_rows<H>(m, row, m.rowStride);
 #pragma unroll
-      for (int j = 0; j < KU; j++) {
+      for (int j = 0; j < H; j++) {
         if (row[j] < 0) continue;
         const unsigned char* y = m.row + (long long)row[j] * m.rowStride;
         b[j].raw = ANY ? load_word<T>(y, lo, bytes, near) : load_16(y + lo);
       }
 #pragma unroll
-      for (int j = 0; j < KU; j++) {
+      for (int j = 0; j < H; j++) {
         if (row[j] < 0) continue;
         if (ANY) b[j].raw = join_words(b[j].raw, m.row + (long long)row[j] * m.rowStride, lo);
 #pragma unroll
@@ -495,10 +512,13 @@ cudaError_t gather(const RowsMove& m, int numSM, cudaStream_t stream) {
     if (threads == 128) return launch_row_kernel(gather_kernel<T, ANY, KU, 128, true>, g, 128, 0, 0, stream, m);
     return launch_row_kernel(gather_kernel<T, ANY, KU, 64, true>, g, 64, 0, 0, stream, m);
   }
-  const int threads = few || vecs >= 512 ? 128 : 64;
-  const dim3 g = token_grid(m, vecs, threads, few);
-  if (threads == 128) return launch_row_kernel(gather_kernel<T, ANY, KU, 128, false>, g, 128, 0, 0, stream, m);
-  return launch_row_kernel(gather_kernel<T, ANY, KU, 64, false>, g, 64, 0, 0, stream, m);
+  if constexpr (KU <= 8) {
+    const int threads = few || vecs >= 512 ? 128 : 64;
+    const dim3 g = token_grid(m, vecs, threads, few);
+    if (threads == 128) return launch_row_kernel(gather_kernel<T, ANY, KU, 128, false>, g, 128, 0, 0, stream, m);
+    return launch_row_kernel(gather_kernel<T, ANY, KU, 64, false>, g, 64, 0, 0, stream, m);
+  }
+  return cudaErrorInvalidValue;          // sixteen at a time only with the weights' gradient: move_rows
 }
 
 template <typename T, bool ANY>
@@ -511,6 +531,9 @@ cudaError_t move_rows(const RowsMove& m, bool rowsOut, int pad, int numSM, cudaS
   }
   if constexpr (sizeof(T) > 1) {
     if (m.choices <= 4) return gather<T, ANY, 4>(m, numSM, stream);
+    // Up to 16 rows in one walk with the weights' gradient: sums of 10 rows of 4 KB for 8192 tokens took 135 us
+    // in a walk for the gradient and one for the sums, 110 in one.
+    if (m.choices > 8 && m.dweight) return gather<T, ANY, 16>(m, numSM, stream);
     return gather<T, ANY, 8>(m, numSM, stream);
   }
   return cudaErrorInvalidValue;          // bytes are not summed: check_rows_move

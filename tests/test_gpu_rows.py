@@ -581,6 +581,35 @@ def test_capture_behind_copies_and_other_streams(native):
         assert (rows[r.want[1][-1]:] == 0).all()
 
 
+def test_waits_for_events_of_other_streams(native):
+    """A call behind an event of another stream, with this stream's own kernels just before it."""
+    import torch
+    side, other = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        r = Run(native, routing(3000, 4, 30, 1), 64, "f32", 30, align=4)
+    x, rows, out = torch.zeros(3000, 64, device="cuda"), torch.zeros(r.r, 64, device="cuda"), torch.zeros(3000, 64, device="cuda")
+    ids = [routing(3000, 4, 30, k).int().cuda() for k in range(2, 6)]
+    wrong = torch.zeros(1, dtype=torch.int64, device="cuda")
+    torch.cuda.synchronize()
+    for i, new in enumerate(ids * 3):
+        with torch.cuda.stream(side):
+            r.sort()
+        other.wait_stream(side)
+        with torch.cuda.stream(other):
+            torch.cuda._sleep(1000000)
+            r.ids.copy_(new)
+            x.fill_(float(i))
+        with torch.cuda.stream(side):
+            r.plan.combine(rows.data_ptr(), r.row_of.data_ptr(), out.data_ptr())      # overlaps the other stream
+            side.wait_stream(other)
+            r.sort()
+            r.plan.dispatch(x.data_ptr(), *r.maps(), rows.data_ptr())
+            r.plan.combine(rows.data_ptr(), r.row_of.data_ptr(), out.data_ptr())
+            wrong += (out != 4.0 * i).any() + (r.count != torch.bincount(new.view(-1).long(), minlength=30)).any()
+    torch.cuda.synchronize()
+    assert wrong.item() == 0
+
+
 def test_one_plan_from_several_threads(native):
     import threading
     import torch
