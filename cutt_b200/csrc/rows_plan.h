@@ -166,16 +166,24 @@ constexpr int kPagedItems = 4;         // accesses of a thread in flight at once
 // strides in bytes; addresses: those of all rows and caches, or-ed together.
 PagedItems paged_items(const PagedShape& s, long long tokenStride, long long headStride, unsigned long long addresses);
 
-// Access i of a block whose first token is q0: byte offsets in the cache and in the rows.  False where
-// the token's slot is not one of the cache's.
-CUTT_HD bool paged_item(const PagedItems& p, const long long* slot, int q0, uint32_t i, long long& cache, long long& row) {
+// Access i of a block whose first token is q0: its token, head and place in the head's elements.
+struct PagedPlace {
+  int token;
+  uint32_t head, piece;
+};
+CUTT_HD PagedPlace paged_place(const PagedItems& p, int q0, uint32_t i) {
   const uint32_t q = fdiv(i, p.divRow), r = i - q * (uint32_t)p.vecs;
-  const uint32_t h = fdiv(r, p.divHead), v = r - h * p.divHead.d;
-  const long long at = cache_offset(p.s, slot[q0 + q], p.divPage);
-  if (at < 0) return false;
-  cache = (at + (long long)h * p.s.headStride) * p.s.elt + (long long)v * p.access;
-  row = (long long)(q0 + q) * p.tokenStride + (long long)h * p.headStride + (long long)v * p.access;
-  return true;
+  const uint32_t h = fdiv(r, p.divHead);
+  return PagedPlace{q0 + (int)q, h, r - h * p.divHead.d};
+}
+// Its byte offset in the rows.
+CUTT_HD long long paged_row(const PagedItems& p, const PagedPlace& a) {
+  return (long long)a.token * p.tokenStride + a.head * p.headStride + (long long)a.piece * p.access;
+}
+// Its byte offset in the cache; -1 where the token's slot is not one of the cache's.
+CUTT_HD long long paged_cache(const PagedItems& p, const PagedPlace& a, long long slot) {
+  const long long at = cache_offset(p.s, slot, p.divPage);
+  return at < 0 ? -1 : (at + a.head * p.s.headStride) * p.s.elt + (long long)a.piece * p.access;
 }
 
 }  // namespace cuttb
