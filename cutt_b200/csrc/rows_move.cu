@@ -172,16 +172,17 @@ __device__ __forceinline__ void block_sums(float (&v)[K], float* dweight, int n,
   __syncthreads();
 }
 
-// Rows (-1: dropped) and weights of the slots j0 .. j0+KU-1 of a token.
+// Rows (-1: dropped) and weights of the slots j0 .. j0+KU-1 of a token.  All loads are issued before the
+// first is looked at; a dropped slot's weight is read with the others and not used.
 template <int KU>
 __device__ __forceinline__ void load_slots(const RowsMove& m, long long s0, int j0, int (&row)[KU], float (&w)[KU]) {
 #pragma unroll
-  for (int j = 0; j < KU; j++) {
-    row[j] = j0 + j < m.choices ? m.rowOf[s0 + j0 + j] : -1;
-    if ((unsigned)row[j] >= (unsigned)m.capacity) row[j] = -1;
-  }
+  for (int j = 0; j < KU; j++) row[j] = j0 + j < m.choices ? m.rowOf[s0 + j0 + j] : -1;
 #pragma unroll
-  for (int j = 0; j < KU; j++) w[j] = m.weight && row[j] >= 0 ? m.weight[s0 + j0 + j] : 1.f;
+  for (int j = 0; j < KU; j++) w[j] = m.weight && j0 + j < m.choices ? m.weight[s0 + j0 + j] : 1.f;
+#pragma unroll
+  for (int j = 0; j < KU; j++)
+    if ((unsigned)row[j] >= (unsigned)m.capacity) row[j] = -1;
 }
 
 template <int KU>
@@ -241,6 +242,11 @@ scatter_kernel(const __grid_constant__ RowsMove m, int padBlocks) {
   const int misX = ANY ? (int)((uintptr_t)x & 15) : 0;
   const bool nearX = ANY && near_end(t, m.tokens, m.tokenStride);
   const long long s0 = (long long)t * m.choices;
+  // the first piece is on its way while the slots are looked up
+  bool ahead = true;
+  uint4 early = make_uint4(0, 0, 0, 0);
+  if (ANY) early = load_word<T>(x, (v0 + first) * 16 - misX, bytes, nearX);
+  else if (v0 + first < v1) early = load_16(x + (v0 + first) * 16);
   for (int j0 = 0; j0 < m.choices; j0 += KU) {
     int row[KU];
     float w[KU], dot[KU];
@@ -251,8 +257,10 @@ scatter_kernel(const __grid_constant__ RowsMove m, int padBlocks) {
     for (int v = v0 + first; ANY ? __any_sync(0xffffffffu, !lender && v < v1) : v < v1; v += STEP) {
       Piece<T> a, o[DOT ? KU : 1];
       uint4 below, here, above;
-      if (ANY) here = load_word<T>(x, v * 16 - misX, bytes, nearX);
-      else a.raw = load_16(x + v * 16);
+      if (ahead) here = early;
+      else here = ANY ? load_word<T>(x, v * 16 - misX, bytes, nearX) : load_16(x + v * 16);
+      ahead = false;
+      if (!ANY) a.raw = here;
       if (DOT) {
 #pragma unroll
         for (int j = 0; j < KU; j++) {
