@@ -198,9 +198,10 @@ __device__ __forceinline__ bool near_rows(const RowsMove& m, const int (&row)[KU
 // with the weights' gradient (16384 tokens, half of 8 slots dropped, 4 KB) 24 warps 110, 32 warps 124;
 // 16384 tokens to 8 rows of 2001 bf16 with 32, 48, 64 warps 119, 126, 132; sums of 8 rows of 4 KB, half
 // dropped, 24, 28, 32 warps 60, 57, 59; sums of 4 rows of 5 KB 32, 40, 48 warps 36.2, 35.2, 35.5; sums of 10
-// rows of 4 KB with the weights' gradient 16, 20, 24 warps 171, 110, 139.
+// rows of 4 KB with the weights' gradient 16, 20, 24 warps 171, 110, 139; of 3 rows of 1111 fp32 with it (1023
+// tokens) 32, 40 warps 8.4, 10.4.
 constexpr int scatter_warps(bool, bool dot) { return dot ? 24 : 32; }
-constexpr int gather_warps(int ku) { return ku > 8 ? 20 : ku > 4 ? 28 : 40; }
+constexpr int gather_warps(int ku, bool dot) { return ku > 8 ? 20 : ku > 4 ? 28 : dot ? 32 : 40; }
 
 // ANY: rows at any address; the pieces of a row are then cut at the 16-byte boundaries of the row
 // that is written, so its first and last pieces may be partial.  The token's words are cut at its
@@ -313,7 +314,7 @@ scatter_kernel(const __grid_constant__ RowsMove m, int padBlocks) {
 }
 
 template <typename T, bool ANY, int KU, int THREADS, bool DOT>
-__global__ void __launch_bounds__(THREADS, gather_warps(KU) * 32 / THREADS)
+__global__ void __launch_bounds__(THREADS, gather_warps(KU, DOT) * 32 / THREADS)
 gather_kernel(const __grid_constant__ RowsMove m) {
   __shared__ float part[THREADS / 32][KU];
   begin_row_kernel();
