@@ -9,6 +9,7 @@ Device code is compiled for sm_100a only.
 """
 from __future__ import annotations
 
+import concurrent.futures
 import os
 import shutil
 import subprocess
@@ -63,20 +64,19 @@ def build(force: bool = False, verbose: bool = False) -> dict:
     def deps(src):
         return hdrs + (rows_hdrs if src in ROWS_SOURCES else [])
     with open(os.path.join(OBJDIR, "build.log"), "a") as log:
-        for src in CU_SOURCES:
+        todo = []
+        for src in CU_SOURCES + CXX_SOURCES:
             s = os.path.join(CSRC, src)
             o = os.path.join(OBJDIR, src + ".o")
             if force or _newer(o, [s] + deps(src)):
-                out = _run([NVCC] + NVCC_FLAGS + ["-c", s, "-o", o], log)
+                tool = [NVCC] + NVCC_FLAGS if src in CU_SOURCES else ["g++"] + CXX_FLAGS
+                todo.append(tool + ["-c", s, "-o", o])
+            objs.append(o)
+        # the sources do not depend on one another: half a minute to two for some of them
+        with concurrent.futures.ThreadPoolExecutor(os.cpu_count() or 1) as pool:
+            for out in pool.map(lambda cmd: _run(cmd, log), todo):
                 if verbose:
                     print(out)
-            objs.append(o)
-        for src in CXX_SOURCES:
-            s = os.path.join(CSRC, src)
-            o = os.path.join(OBJDIR, src + ".o")
-            if force or _newer(o, [s] + deps(src)):
-                _run(["g++"] + CXX_FLAGS + ["-c", s, "-o", o], log)
-            objs.append(o)
         so = os.path.join(LIBDIR, "libcutt.so")
         if force or _newer(so, objs):
             _run([NVCC, "-shared", "-o", so] + objs + GENCODE, log)
