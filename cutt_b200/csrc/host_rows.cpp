@@ -68,7 +68,7 @@ long long cutt_hostcheck_pages_run(int requests, int pageSize, int tableWidth, i
     tokens += added[b] > 0 ? added[b] : 0;
     if (freeList) {
       pageOffset[b] = (int)pages;
-      pages += pages_taken(held[b], added[b], pageSize, tableWidth);
+      pages += pages_taken(held[b], added[b], p.s.divPage, tableWidth);
     }
   }
   tokenOffset[requests] = saturate(tokens);
@@ -90,7 +90,7 @@ long long cutt_hostcheck_pages_run(int requests, int pageSize, int tableWidth, i
     for (int f = pageOffset[0]; f < pageOffset[requests]; f++) {
       const int b = last_at_or_before(pageOffset, requests + 1, f);
       if (b < 0 || b >= requests) { bad++; continue; }
-      const long long idx = pages_of(held[b] > 0 ? held[b] : 0, pageSize) + (long long)(f - pageOffset[b]);
+      const long long idx = pages_of(held[b] > 0 ? held[b] : 0, p.s.divPage) + (long long)(f - pageOffset[b]);
       if (idx >= tableWidth) { bad++; continue; }
       take_page(p, b, f, limit);
     }

@@ -75,7 +75,7 @@ __device__ __forceinline__ uint2 scan_requests(const PagesBuild& p, const Pool& 
     const int b = b0 + threadIdx.x;
     const bool in = b < p.s.requests;
     const int n = in ? max(0, p.added[b]) : 0;
-    const int g = in && p.freeList ? pages_taken(p.held[b], n, p.s.pageSize, p.s.tableWidth) : 0;
+    const int g = in && p.freeList ? pages_taken(p.held[b], n, p.s.divPage, p.s.tableWidth) : 0;
     uint2 total;
     const uint2 at = block_scan2(make_uint2(n, g), s, total);
     if (in) {

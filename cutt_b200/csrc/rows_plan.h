@@ -78,14 +78,13 @@ CUTT_HD int clip_row(int o, int capacity) { return o < capacity ? o : capacity; 
 CUTT_HD int held_rows(int o, int n, int capacity) { return clip_row(o + n, capacity) - clip_row(o, capacity); }
 CUTT_HD int align_rows(int n, int align) { return (n + align - 1) / align * align; }
 
-// Pages of a request: held by its tokens, taken for the new ones.
-CUTT_HD unsigned pages_of(unsigned long long tokens, unsigned pageSize) {
-  return (unsigned)((tokens + pageSize - 1) / pageSize);
-}
-CUTT_HD int pages_taken(int held, int added, int pageSize, int tableWidth) {
-  const unsigned c = held > 0 ? held : 0, n = added > 0 ? added : 0;
-  const unsigned have = pages_of(c, pageSize), all = pages_of((unsigned long long)c + n, pageSize);
-  const unsigned want = all < (unsigned)tableWidth ? all : tableWidth;
+// Pages of a request: held by its tokens, taken for the new ones.  Lengths are at most 2^31 - 1 each, so
+// their sum has 32 bits (a 64-bit division would take longer than everything else on a request).
+CUTT_HD uint32_t pages_of(uint32_t tokens, const FastDiv& divPage) { return tokens ? fdiv(tokens - 1, divPage) + 1 : 0; }
+CUTT_HD int pages_taken(int held, int added, const FastDiv& divPage, int tableWidth) {
+  const uint32_t c = held > 0 ? held : 0, n = added > 0 ? added : 0;
+  const uint32_t have = pages_of(c, divPage), all = pages_of(c + n, divPage);
+  const uint32_t want = all < (uint32_t)tableWidth ? all : tableWidth;
   return want > have ? (int)(want - have) : 0;
 }
 
@@ -123,7 +122,7 @@ CUTT_HD long long slot_of_token(const PagesBuild& p, int b, int q, int limit) {
   const unsigned idx = fdiv(pos, p.s.divPage);
   if (idx >= (unsigned)p.s.tableWidth) return -1;
   int page;
-  const unsigned have = p.freeList ? pages_of(c, p.s.pageSize) : 0xffffffffu;
+  const unsigned have = p.freeList ? pages_of(c, p.s.divPage) : 0xffffffffu;
   if (idx < have) {
     page = p.table[(long long)b * p.tableStride + idx];
   } else {
@@ -136,7 +135,7 @@ CUTT_HD long long slot_of_token(const PagesBuild& p, int b, int q, int limit) {
 // Writes the table entry of position f of the free list (pageOffset[0] <= f < pageOffset[requests]).
 CUTT_HD void take_page(const PagesBuild& p, int b, int f, int limit) {
   const unsigned c = p.held[b] > 0 ? p.held[b] : 0;
-  const unsigned idx = pages_of(c, p.s.pageSize) + (unsigned)(f - p.pageOffset[b]);
+  const unsigned idx = pages_of(c, p.s.divPage) + (unsigned)(f - p.pageOffset[b]);
   p.table[(long long)b * p.tableStride + idx] = f < limit ? p.freeList[f] : -1;
 }
 
