@@ -116,9 +116,8 @@ long long cutt_hostcheck_paged_run(const int* shape, const long long* strides, l
     const int nq = p.perBlock < s.tokens - q0 ? p.perBlock : s.tokens - q0;
     for (uint32_t i = 0; i < (uint32_t)nq * p.vecs; i++) {
       const PagedPlace a = paged_place(p, q0, i);
-      const long long c = paged_cache(p, a, slot[a.token]), r = paged_row(p, a);
-      if (r < 0 || r + p.access > rowBytes) bad++;       // rows to be stored are read whatever their slot
-      if (c < 0) continue;
+      long long r, c;
+      if (!paged_access(p, a, slot[a.token], r, c)) continue;
       if (c < 0 || r < 0 || c + p.access > cacheBytes || r + p.access > rowBytes || (uintptr_t)(cache + c) % p.access ||
           (uintptr_t)(rows + r) % p.access) {
         bad++;

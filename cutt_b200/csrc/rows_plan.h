@@ -175,14 +175,14 @@ CUTT_HD PagedPlace paged_place(const PagedItems& p, int q0, uint32_t i) {
   const uint32_t h = fdiv(r, p.divHead);
   return PagedPlace{q0 + (int)q, h, r - h * p.divHead.d};
 }
-// Its byte offset in the rows.
-CUTT_HD long long paged_row(const PagedItems& p, const PagedPlace& a) {
-  return (long long)a.token * p.tokenStride + a.head * p.headStride + (long long)a.piece * p.access;
-}
-// Its byte offset in the cache; -1 where the token's slot is not one of the cache's.
-CUTT_HD long long paged_cache(const PagedItems& p, const PagedPlace& a, long long slot) {
+// Its byte offsets in the rows and in the cache.  False where the token's slot is not one of the cache's:
+// neither side is read or written then (the rows may end before such a token).
+CUTT_HD bool paged_access(const PagedItems& p, const PagedPlace& a, long long slot, long long& row, long long& cache) {
   const long long at = cache_offset(p.s, slot, p.divPage);
-  return at < 0 ? -1 : (at + a.head * p.s.headStride) * p.s.elt + (long long)a.piece * p.access;
+  if (at < 0) return false;
+  row = (long long)a.token * p.tokenStride + a.head * p.headStride + (long long)a.piece * p.access;
+  cache = (at + a.head * p.s.headStride) * p.s.elt + (long long)a.piece * p.access;
+  return true;
 }
 
 }  // namespace cuttb

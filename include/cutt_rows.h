@@ -117,8 +117,8 @@ int cutt_pages_plan_rows(unsigned int* handle, int tokens, int heads, int headSi
 
 /* Stores rows into / loads rows from the slots slot[tokens].  Row q, head h starts at q *
  * tokenStride + h * headStride (elements; for loads both at least headSize).  v and vCache may
- * both be NULL.  Rows whose slot is not in 0 .. pages * pageSize - 1 are skipped: the cache, or
- * the row, is left alone.  Two rows stored to one slot leave either's elements there. */
+ * both be NULL.  Rows whose slot is not in 0 .. pages * pageSize - 1 are skipped: neither the cache
+ * nor the row is read or written (k and v may end before such rows).  Two rows stored to one slot leave either's elements there. */
 int cutt_pages_store(unsigned int handle, const void* k, const void* v, long long tokenStride,
                      long long headStride, const long long* slot, void* kCache, void* vCache);
 int cutt_pages_load(unsigned int handle, const void* kCache, const void* vCache, const long long* slot,

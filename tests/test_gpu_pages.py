@@ -212,6 +212,24 @@ def test_store_and_load(native, elt, heads, size, page, head_major, pad):
         k, v = v, k
 
 
+@pytest.mark.parametrize("size", [64, 33])
+def test_rows_end_before_skipped_tokens(native, size):
+    """A batch shorter than the plan's tokens: the slots behind its last row are -1."""
+    import torch
+    n, have, pages, page, heads = 300, 37, 9, 8, 4
+    cache = torch.zeros(pages, page, heads, size, device="cuda")
+    k = torch.randn(have, heads, size, device="cuda")
+    slot = torch.full((n,), -1, dtype=torch.int64, device="cuda")
+    slot[:have] = torch.randperm(pages * page, device="cuda")[:have]
+    p = native.PagedRows(n, heads, size, 4, pages, page, *cache.stride()[:3], stream=torch.cuda.current_stream().cuda_stream)
+    p.store(k.data_ptr(), 0, slot.data_ptr(), cache.data_ptr(), 0)
+    flat = cache.view(pages * page, heads, size)
+    assert torch.equal(flat[slot[:have]], k) and flat.abs().sum((1, 2)).count_nonzero() == have
+    back = torch.zeros_like(k)
+    p.load(cache.data_ptr(), 0, slot.data_ptr(), back.data_ptr(), 0)
+    assert torch.equal(back, k)
+
+
 def test_one_row_to_many_slots_and_no_tokens(native):
     import torch
     cache = torch.zeros(4, 8, 2, 16, device="cuda")

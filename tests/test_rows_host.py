@@ -334,3 +334,28 @@ def test_paged_accesses_on_the_host(hc, elt, heads, size, page, head_major, pad,
                                            flat.ctypes.data, flat.nbytes, store) == 0
         assert np.array_equal(view, want_cache) and np.array_equal(r3, want_rows)
         rows[:] = rng.integers(0, 250, rows.size)
+
+
+@pytest.mark.parametrize("elt,heads,size", [(2, 8, 128), (4, 3, 33), (1, 5, 1)])
+def test_skipped_tokens_need_no_rows(hc, elt, heads, size):
+    """Rows that end before the tokens whose slots are -1 or beyond the cache: nothing behind the end is touched."""
+    pages, page, n, have = 6, 8, 40, 23
+    dt = {1: np.uint8, 2: np.uint16, 4: np.uint32}[elt]
+    rng = np.random.default_rng(size)
+    cache = rng.integers(0, 250, (pages * page, heads, size)).astype(dt)
+    rows = rng.integers(0, 250, (have, heads, size)).astype(dt)
+    slot = np.full(n, -1, np.int64)
+    slot[:have] = rng.permutation(pages * page)[:have]
+    slot[have + 1], slot[have + 2] = pages * page, 2**50
+    strides = (ctypes.c_longlong * 3)(page * heads * size, heads * size, size)
+    ints = _ints(n, heads, size, elt, pages, page)
+    for store in (1, 0):
+        want_cache, want_rows = cache.copy(), rows.copy()
+        if store:
+            want_cache[slot[:have]] = rows
+        else:
+            want_rows[:] = cache[slot[:have]]
+        assert hc.cutt_hostcheck_paged_run(ints, strides, heads * size, size, slot.ctypes.data, rows.ctypes.data, rows.nbytes,
+                                           cache.ctypes.data, cache.nbytes, store) == 0
+        assert np.array_equal(cache, want_cache) and np.array_equal(rows, want_rows)
+        rows[:] = rng.integers(0, 250, rows.shape)
