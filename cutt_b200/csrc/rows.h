@@ -10,9 +10,11 @@ namespace cuttb {
 // Launch of a row operator's kernel.  The kernels of a step follow one another in microseconds, so each
 // is launched while the one before it still runs (programmatic dependent launch) and waits, as its first
 // statement, for that one's end: begin_row_kernel.  It lets the next kernel start in turn only then, so
-// whatever precedes this kernel in the stream is done before the next one begins, and a kernel may read
-// this one's INPUTS before it waits itself.  Inputs are read with coherent loads (no __restrict__): a line
-// may have come into the cache before the kernel that writes it ended.
+// whatever precedes this kernel in the stream is done before the next one begins.  Within the map of three
+// kernels (rows_map.cu) two differ: sort_starts lets sort_rows start before its own wait, and sort_rows
+// ranks the map's inputs before its wait, with loads that allow that (load_index there).  Inputs are read
+// with coherent loads (no __restrict__): a line may have come into the cache before the kernel that writes
+// it ended.
 // `cluster`: blocks of a cluster, 0 for none.
 template <typename... P, typename... A>
 cudaError_t launch_row_kernel(void (*kernel)(P...), dim3 grid, int threads, size_t smem, int cluster, cudaStream_t stream, A... args) {

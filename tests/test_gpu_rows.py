@@ -543,6 +543,26 @@ def test_steps_without_a_pause(native, t, e, steps):
     assert wrong.item() == 0          # sums of 4 and 16 equal numbers are exact
 
 
+@pytest.mark.parametrize("wide", [False, True])
+def test_long_map_of_indices_written_just_before(native, wide):
+    """The map in three kernels: its last one reads the indices before it waits for the others.  Every step
+    writes other indices with a kernel right before the map, where the step before left its own in the caches."""
+    import torch
+    n, e = 300000, 256
+    r = Run(native, torch.zeros(n, 1, dtype=torch.int64), 8, "bf16", e, align=16, index=torch.int64 if wide else torch.int32)
+    base = torch.randint(0, e, (n, 1), device="cuda").to(r.ids.dtype)
+    wrong = torch.zeros(1, dtype=torch.int64, device="cuda")
+    slots = torch.arange(n, device="cuda").view(n, 1)
+    for i in range(150):
+        torch.remainder(base + i * 37, e, out=r.ids)
+        r.sort()
+        row = r.row_of.view(-1).long()
+        expert = torch.searchsorted(r.offset[1:].contiguous(), r.row_of.view(-1), right=True)      # of the segment of each slot's row
+        wrong += (expert != r.ids.view(-1)).any() + (r.slot_of[row].view(n, 1) != slots).any()
+        wrong += (r.count != torch.bincount(r.ids.view(-1).long(), minlength=e)).any()
+    assert wrong.item() == 0
+
+
 def test_capture_behind_copies_and_other_streams(native):
     """Graph nodes before the operators that are not kernels (copies, a fill), and a join with another stream."""
     import torch
