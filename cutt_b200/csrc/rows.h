@@ -16,10 +16,13 @@ namespace cuttb {
 // with coherent loads (no __restrict__): a line may have come into the cache before the kernel that writes
 // it ended.
 // `cluster`: blocks of a cluster, 0 for none.
+// The limit of a kernel's shared memory belongs to the process, and calls of several threads need different
+// sizes of one kernel: every call sets the same limit, which is enough for all of them.
+constexpr int kRowSharedLimit = 220 * 1024;   // an SM's 227 KB less what the kernels declare statically
 template <typename... P, typename... A>
 cudaError_t launch_row_kernel(void (*kernel)(P...), dim3 grid, int threads, size_t smem, int cluster, cudaStream_t stream, A... args) {
   if (smem > 40 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowSharedLimit);
     if (e != cudaSuccess) return e;
   }
   if (cluster > 8) {

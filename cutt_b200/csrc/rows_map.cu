@@ -428,6 +428,7 @@ constexpr int kBlockSlots = 512;
 constexpr int kBlockWarps = 16;
 
 constexpr int kMostWords = 216 * 1024 / 4;   // of a block's shared memory
+static_assert(kMostWords * 4 <= kRowSharedLimit, "every call's shared memory is within the limit that all calls set");
 
 // Warps of a block whose histograms leave room for `slots` slots.
 int warps_for(int slots, int experts, int most) {

@@ -661,6 +661,55 @@ def test_one_plan_from_several_threads(native):
         assert torch.equal(out, 4 * x)
 
 
+@pytest.mark.parametrize("tokens", [(1024, 8192), (20000, 60000)])
+def test_sorts_of_several_sizes_from_several_threads(native, tokens):
+    """Two threads whose maps need different amounts of one kernel's shared memory."""
+    import threading
+    import torch
+    runs, failed = [], []
+    for t in tokens:
+        with torch.cuda.stream(torch.cuda.Stream()):
+            runs.append(Run(native, routing(t, 8, 256, t), 8, "bf16", 256, align=8))
+    torch.cuda.synchronize()
+
+    def work(r):
+        torch.cuda.set_device(0)
+        for _ in range(3000):
+            try:
+                r.sort()
+            except native.CuttError as e:
+                failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(r,)) for r in runs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not failed
+    for r in runs:
+        r.check_map()
+
+
+@pytest.mark.parametrize("order", [(0, 1), (1, 0)])
+def test_sorts_of_several_sizes_in_one_graph(native, order):
+    """A graph is instantiated after all its calls were captured, the smaller maps among them."""
+    import torch
+    side, runs = torch.cuda.Stream(), []
+    with torch.cuda.stream(side):
+        for t in (1024, 8192):
+            runs.append(Run(native, routing(t, 8, 256, t), 8, "bf16", 256, align=8))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        for i in order:
+            runs[i].sort()
+    graph.replay()
+    torch.cuda.synchronize()
+    for r in runs:
+        r.check_map()
+
+
 def test_calls_on_another_device_are_refused(native):
     import torch
     if torch.cuda.device_count() < 2:
