@@ -130,6 +130,15 @@ long long cutt_hostcheck_paged_run(const int* shape, const long long* strides, l
   return bad;
 }
 
+// {blocks, slots, warps, words} of the map's launch.
+void cutt_hostcheck_sort_shape(int n, int experts, int most, int* out) {
+  const SortShape c = sort_shape(n, experts, most);
+  out[0] = c.blocks;
+  out[1] = c.slots;
+  out[2] = c.warps;
+  out[3] = c.words;
+}
+
 int cutt_hostcheck_local_expert(long long e, int first, int experts) { return local_expert(e, first, experts); }
 
 }  // extern "C"

@@ -132,7 +132,6 @@ __device__ __forceinline__ void expand_requests(const PagesBuild& p, int limit, 
 // pool is updated in place (`inPlace`): then the blocks are one cluster, and the pool is written
 // after all of them have read it.
 constexpr int kSharedRequests = 4096;
-constexpr int kMostBlocks = 16;
 
 __global__ void __launch_bounds__(1024)
 pages_build(const __grid_constant__ PagesBuild p, const int* poolIn, int* poolOut, int* tokenOffset, int* pageOffset, bool inPlace) {
@@ -256,15 +255,28 @@ constexpr int kBlockTokens = 1024;
 // 8192 tokens 6.1 against 7.4 us, 131072 tokens 12.6 against 6.8 us.
 constexpr int kClusterTokens = 16384;
 
+// Blocks and threads of the one kernel.
+int build_blocks(const PagesShape& s, int most) {
+  int blocks = 1;
+  while (blocks * 2 <= most && s.maxTokens > blocks * kBlockTokens) blocks *= 2;
+  return blocks;
+}
+int build_threads(const PagesShape& s) { return s.requests > 512 || s.maxTokens > 512 ? 1024 : 512; }
+
+int pages_build_clusters(const PagesShape& s, cudaStream_t stream) {
+  if (s.requests > kSharedRequests || s.maxTokens > kClusterTokens) return kMostClusterBlocks;     // two kernels
+  const int blocks = build_blocks(s, kMostClusterBlocks);
+  return blocks <= kPortableBlocks || cluster_fits(pages_build, blocks, build_threads(s), 8 * (s.requests + 1), stream) ? kMostClusterBlocks
+                                                                                                                     : kPortableBlocks;
+}
+
 cudaError_t launch_pages_build(const PagesBuild& b, const int* poolIn, int* poolOut, int* tokenOffset, int* pageOffset,
-                               int numSM, cudaStream_t stream) {
+                               int numSM, int cluster, cudaStream_t stream) {
   const bool inPlace = b.freeList && poolIn == poolOut;
   if (b.s.requests <= kSharedRequests && (!inPlace || b.s.maxTokens <= kClusterTokens)) {
-    int blocks = 1;
-    const int most = inPlace ? kMostBlocks : numSM;
-    while (blocks * 2 <= most && b.s.maxTokens > blocks * kBlockTokens) blocks *= 2;
-    return launch_row_kernel(pages_build, dim3(blocks), b.s.requests > 512 || b.s.maxTokens > 512 ? 1024 : 512,
-                             8 * (b.s.requests + 1), inPlace ? blocks : 0, stream, b, poolIn, poolOut, tokenOffset, pageOffset, inPlace);
+    const int blocks = build_blocks(b.s, inPlace ? cluster : numSM);
+    return launch_row_kernel(pages_build, dim3(blocks), build_threads(b.s), 8 * (b.s.requests + 1), inPlace ? blocks : 0, stream, b, poolIn,
+                             poolOut, tokenOffset, pageOffset, inPlace);
   }
   const cudaError_t e = launch_row_kernel(pages_scan, dim3(1), 1024, 0, 0, stream, b, poolIn, poolOut, tokenOffset, pageOffset);
   if (e != cudaSuccess) return e;

@@ -49,6 +49,31 @@ cudaError_t launch_row_kernel(void (*kernel)(P...), dim3 grid, int threads, size
   return e;
 }
 
+// Whether the device, or the part of it that the stream's context has (a green context), can hold a cluster of
+// this launch.  Clusters of up to kPortableBlocks blocks fit everywhere; larger ones are asked for when the plan
+// is made.
+template <typename... P>
+bool cluster_fits(void (*kernel)(P...), int blocks, int threads, size_t smem, cudaStream_t stream) {
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = blocks;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cudaLaunchConfig_t c{};
+  c.gridDim = dim3(blocks);
+  c.blockDim = dim3(threads);
+  c.dynamicSmemBytes = smem;
+  c.stream = stream;
+  c.attrs = &attr;
+  c.numAttrs = 1;
+  int n = 0;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowSharedLimit) == cudaSuccess &&
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) == cudaSuccess &&
+      cudaOccupancyMaxActiveClusters(&n, kernel, &c) == cudaSuccess)
+    return n > 0;
+  cudaGetLastError();
+  return false;
+}
+
 #ifdef __CUDACC__
 __device__ __forceinline__ void begin_row_kernel() {
   cudaGridDependencySynchronize();
@@ -56,8 +81,11 @@ __device__ __forceinline__ void begin_row_kernel() {
 }
 #endif
 
+// `cluster`: most blocks of a cluster, as rows_sort_clusters (pages_build_clusters) says for the plan's stream.
+int rows_sort_clusters(const RowsShape& s, cudaStream_t stream);
+int pages_build_clusters(const PagesShape& s, cudaStream_t stream);
 cudaError_t launch_rows_sort(const RowsShape& s, const void* expertOf, int indexBytes, int* count, int* offset,
-                             int* rowOf, int* slotOf, int numSM, cudaStream_t stream);
+                             int* rowOf, int* slotOf, int numSM, int cluster, cudaStream_t stream);
 
 // One row to its slots' rows (dispatch, combine_grad) and the sum of its slots' rows (combine,
 // dispatch_grad).  token / row: the tensors of the two sides, whichever is written.
@@ -77,7 +105,7 @@ cudaError_t launch_rows_scatter(const RowsMove& m, int align, int numSM, cudaStr
 cudaError_t launch_rows_gather(const RowsMove& m, int numSM, cudaStream_t stream);
 
 cudaError_t launch_pages_build(const PagesBuild& b, const int* poolIn, int* poolOut, int* tokenOffset, int* pageOffset,
-                               int numSM, cudaStream_t stream);
+                               int numSM, int cluster, cudaStream_t stream);
 
 struct PagedMove {
   const unsigned char* src[2];

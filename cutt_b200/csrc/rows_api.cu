@@ -24,6 +24,7 @@ struct Plan {
   Kind kind;
   int device = 0;
   int numSM = 0;
+  int cluster = 0;         // blocks of the largest cluster that its calls may use
   cudaStream_t stream = 0;
   RowsShape rows{};
   PagesShape pages{};
@@ -42,6 +43,8 @@ int add_plan(unsigned int* handle, Plan& p, void* stream) {
     cudaGetLastError();
     return CUTT_INTERNAL_ERROR;
   }
+  if (p.kind == kRows) p.cluster = rows_sort_clusters(p.rows, p.stream);
+  if (p.kind == kPages) p.cluster = pages_build_clusters(p.pages, p.stream);
   try {
     std::shared_ptr<const Plan> q = std::make_shared<Plan>(p);
     std::lock_guard<std::mutex> lk(g_lock);
@@ -127,11 +130,11 @@ bool rows_describe(unsigned int handle, char* buf, size_t len) {
   static const char* const types[] = {"bytes", "f16", "bf16", "f32"};
   if (p->kind == kRows)
     snprintf(buf, len, "{\"method\": \"rows\", \"tokens\": %d, \"choices\": %d, \"experts\": %d, \"first\": %d, \"align\": %d, "
-             "\"capacity\": %d, \"width\": %d, \"type\": \"%s\"}", p->rows.tokens, p->rows.choices, p->rows.experts,
-             p->rows.first, p->rows.align, p->rows.capacity, p->rows.width, types[p->rows.type]);
+             "\"capacity\": %d, \"width\": %d, \"type\": \"%s\", \"cluster\": %d}", p->rows.tokens, p->rows.choices, p->rows.experts,
+             p->rows.first, p->rows.align, p->rows.capacity, p->rows.width, types[p->rows.type], p->cluster);
   else if (p->kind == kPages)
-    snprintf(buf, len, "{\"method\": \"pages\", \"requests\": %d, \"page_size\": %d, \"table_width\": %d, \"max_tokens\": %d}",
-             p->pages.requests, p->pages.pageSize, p->pages.tableWidth, p->pages.maxTokens);
+    snprintf(buf, len, "{\"method\": \"pages\", \"requests\": %d, \"page_size\": %d, \"table_width\": %d, \"max_tokens\": %d, "
+             "\"cluster\": %d}", p->pages.requests, p->pages.pageSize, p->pages.tableWidth, p->pages.maxTokens, p->cluster);
   else
     snprintf(buf, len, "{\"method\": \"paged rows\", \"tokens\": %d, \"heads\": %d, \"head_size\": %d, \"element\": %d, "
              "\"pages\": %d, \"page_size\": %d}", p->paged.tokens, p->paged.heads, p->paged.headSize, p->paged.elt,
@@ -161,7 +164,7 @@ int cutt_rows_sort(unsigned int handle, const void* expertOf, size_t sizeofIndex
   if (check_rows_sort(p->rows, expertOf, sizeofIndex, count, offset, rowOf, slotOf)) return CUTT_INVALID_PARAMETER;
   const int rc = check_device(*p);
   if (rc != CUTT_SUCCESS) return rc;
-  return result(launch_rows_sort(p->rows, expertOf, (int)sizeofIndex, count, offset, rowOf, slotOf, p->numSM, p->stream));
+  return result(launch_rows_sort(p->rows, expertOf, (int)sizeofIndex, count, offset, rowOf, slotOf, p->numSM, p->cluster, p->stream));
 }
 
 int cutt_rows_dispatch(unsigned int handle, const void* x, long long xStride, const int* rowOf, const int* count,
@@ -203,7 +206,7 @@ int cutt_pages_build(unsigned int handle, const int* held, const int* added, con
   const int rc = check_device(*p);
   if (rc != CUTT_SUCCESS) return rc;
   const PagesBuild b{p->pages, held, added, freeList, poolOut, table, tableStride, tokenOffset, pageOffset, slot};
-  return result(launch_pages_build(b, poolIn, poolOut, tokenOffset, pageOffset, p->numSM, p->stream));
+  return result(launch_pages_build(b, poolIn, poolOut, tokenOffset, pageOffset, p->numSM, p->cluster, p->stream));
 }
 
 int cutt_pages_plan_rows(unsigned int* handle, int tokens, int heads, int headSize, size_t sizeofType, int pages,

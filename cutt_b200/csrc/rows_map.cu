@@ -156,7 +156,6 @@ __device__ __forceinline__ Ranked carve(int* smem, int slots, int warps, int exp
   r.shift = r.total + experts;
   return r;
 }
-int ranked_words(int slots, int warps, int experts) { return 2 * slots + (2 * warps + 2) * experts; }
 
 // Ranks the block's slots lo .. hi-1 and sums the warps' counts: hist becomes, for every warp, the
 // slots of the warps before it, total the block's counts.
@@ -211,9 +210,7 @@ __device__ void write_block(const RowsShape& s, int lo, int hi, const Ranked& r,
   }
 }
 
-constexpr int kMostBlocks = 16;
-
-// The map in one cluster of 1 to kMostBlocks blocks: the blocks read one another's counts through
+// The map in one cluster of 1 to kMostClusterBlocks blocks: the blocks read one another's counts through
 // distributed shared memory, so there is one launch and no workspace.
 template <typename I>
 __global__ void __launch_bounds__(1024)
@@ -239,11 +236,11 @@ sort_cluster(RowsShape s, const I* ids, int slots, int* count, int* offset, int*
     int n_e = 0, before = 0, own = 0;
     if (e < E) {
       own = mine[e];
-      int c[kMostBlocks];                // all reads at once: one after the other each waits for its round trip
+      int c[kMostClusterBlocks];         // all reads at once: one after the other each waits for its round trip
 #pragma unroll
-      for (int b = 0; b < kMostBlocks; b++) c[b] = b < blocks ? cluster.map_shared_rank(mine, b)[e] : 0;
+      for (int b = 0; b < kMostClusterBlocks; b++) c[b] = b < blocks ? cluster.map_shared_rank(mine, b)[e] : 0;
 #pragma unroll
-      for (int b = 0; b < kMostBlocks; b++) {
+      for (int b = 0; b < kMostClusterBlocks; b++) {
         if (b < me) before += c[b];
         n_e += c[b];
       }
@@ -415,42 +412,16 @@ sort_rows(RowsShape s, const I* ids, const int* count, const int* offset, int* r
   fill_gaps(E, s.capacity, count, offset, slotOf, blockIdx.x, gridDim.x);
 }
 
-// Up to this many slots a cluster, above three kernels.  Measured, 128 experts: 32768 slots 6.2
-// against 8.1 us, 65536 slots 7.5 against 8.3 us, and one launch against three; 524288 slots of 256
-// experts take 13 us in three kernels.
-constexpr int kClusterSlots = 65536;
-// A block takes this many slots where one is enough, else half of them, and more once the cluster is
-// full: 512 slots 4.4 us in one block, 4.2 in two; 288 slots 3.8 and 4.5; 1024 slots 4.6 in four, 5.2
-// in two.
-constexpr int kBlockSlots = 512;
-// Warps of a block: one for 32 slots, at most 16 (every further one is a histogram to clear and to
-// scan: 8192 slots per block with 32 warps instead of 16 took 8 us instead of 6).
-constexpr int kBlockWarps = 16;
-
-constexpr int kMostWords = 216 * 1024 / 4;   // of a block's shared memory
-static_assert(kMostWords * 4 <= kRowSharedLimit, "every call's shared memory is within the limit that all calls set");
-
-// Warps of a block whose histograms leave room for `slots` slots.
-int warps_for(int slots, int experts, int most) {
-  int w = most;
-  while (w > 1 && ranked_words(slots, w, experts) + 3 * experts > kMostWords) w >>= 1;
-  return w;
-}
+static_assert(kMostSortWords * 4 <= kRowSharedLimit, "every call's shared memory is within the limit that all calls set");
 
 template <typename I>
 cudaError_t sort_typed(const RowsShape& s, const I* ids, int* count, int* offset, int* rowOf, int* slotOf, int numSM,
-                       cudaStream_t stream) {
+                       int cluster, cudaStream_t stream) {
   const int n = s.tokens * s.choices, E = s.experts;
-  if (n <= kClusterSlots || n < E) {
-    int blocks = 1;
-    if (n > kBlockSlots)
-      while (blocks < kMostBlocks && n > blocks * (kBlockSlots / 2)) blocks <<= 1;
-    const int slots = ((n + blocks - 1) / blocks + 31) & ~31;
-    int warps = warps_for(slots, E, kBlockWarps);
-    while (warps > 4 && warps * 32 > slots) warps >>= 1;
-    return launch_row_kernel(sort_cluster<I>, dim3(blocks), warps * 32, (ranked_words(slots, warps, E) + 3 * E) * 4, blocks, stream, s,
-                             ids, slots, count, offset, rowOf, slotOf);
-  }
+  const SortShape c = sort_shape(n, E, cluster);
+  if (c.blocks)
+    return launch_row_kernel(sort_cluster<I>, dim3(c.blocks), c.warps * 32, c.words * 4, c.blocks, stream, s, ids, c.slots, count, offset,
+                             rowOf, slotOf);
   // one chunk for an SM: more of them are more rows of the table of counts (524288 slots: 148 chunks
   // 15.6 us, 296 chunks 18.5)
   int chunk = (n + numSM - 1) / numSM;
@@ -464,17 +435,26 @@ cudaError_t sort_typed(const RowsShape& s, const I* ids, int* count, int* offset
   if (e != cudaSuccess) return e;
   e = launch_row_kernel(sort_starts, dim3(kStartBlocks), kChunkThreads, 0, 0, stream, s, count, offset, rowOf, chunk, chunks);
   if (e != cudaSuccess) return e;
-  const int warps = warps_for(slots, E, kBlockWarps);
+  const int warps = warps_for(slots, E, kSortWarps);
   return launch_row_kernel(sort_rows<I>, dim3(chunks), warps * 32, ranked_words(slots, warps, E) * 4, 0, stream, s, ids, count,
                            offset, rowOf, slotOf, chunk, chunks, slots);
 }
 
 }  // namespace
 
+int rows_sort_clusters(const RowsShape& s, cudaStream_t stream) {
+  const SortShape c = sort_shape(s.tokens * s.choices, s.experts, kMostClusterBlocks);
+  if (c.blocks <= kPortableBlocks) return kMostClusterBlocks;
+  return cluster_fits(sort_cluster<int>, c.blocks, c.warps * 32, c.words * 4, stream) &&
+                 cluster_fits(sort_cluster<long long>, c.blocks, c.warps * 32, c.words * 4, stream)
+             ? kMostClusterBlocks
+             : kPortableBlocks;
+}
+
 cudaError_t launch_rows_sort(const RowsShape& s, const void* expertOf, int indexBytes, int* count, int* offset,
-                             int* rowOf, int* slotOf, int numSM, cudaStream_t stream) {
-  if (indexBytes == 4) return sort_typed(s, (const int*)expertOf, count, offset, rowOf, slotOf, numSM, stream);
-  return sort_typed(s, (const long long*)expertOf, count, offset, rowOf, slotOf, numSM, stream);
+                             int* rowOf, int* slotOf, int numSM, int cluster, cudaStream_t stream) {
+  if (indexBytes == 4) return sort_typed(s, (const int*)expertOf, count, offset, rowOf, slotOf, numSM, cluster, stream);
+  return sort_typed(s, (const long long*)expertOf, count, offset, rowOf, slotOf, numSM, cluster, stream);
 }
 
 }  // namespace cuttb

@@ -63,6 +63,23 @@ int check_paged_move(const PagedShape& s, const void* k, const void* v, long lon
 // addresses and byte distances, or-ed together.
 int access_bytes(unsigned long long bits, int elt);
 
+// Launch of the map of n slots.  Up to kClusterSlots slots one cluster, above three kernels (blocks = 0).
+// `most`: blocks of the largest cluster that the device can hold, kPortableBlocks at least.
+constexpr int kClusterSlots = 65536;
+constexpr int kMostClusterBlocks = 16;
+constexpr int kPortableBlocks = 8;            // of a cluster that every device can hold
+constexpr int kMostSortWords = 216 * 1024 / 4;   // of a block's shared memory
+// Warps of a block: one for 32 slots, at most 16 (every further one is a histogram to clear and to scan:
+// 8192 slots per block with 32 warps instead of 16 took 8 us instead of 6).
+constexpr int kSortWarps = 16;
+struct SortShape {
+  int blocks, slots, warps;   // of the cluster, of a block, of a block
+  int words;                  // of a block's shared memory
+};
+int ranked_words(int slots, int warps, int experts);
+int warps_for(int slots, int experts, int most);
+SortShape sort_shape(int n, int experts, int most);
+
 // --- index arithmetic ---
 
 // Expert of a slot counted from the first one held here; -1: not held here.

@@ -16,6 +16,9 @@
  * or keeps anything between calls, so every call may be captured into a CUDA graph (a replay
  * reads the maps and lengths that are in the buffers then).
  *
+ * Clusters of 16 blocks are used where the stream's context can hold them, else of 8; a context
+ * must be able to hold those (eight SMs of one group, as the driver splits them for green contexts).
+ *
  * Argument errors return CUTT_INVALID_PARAMETER before anything is launched; a call on another
  * device than the plan's returns CUTT_INVALID_DEVICE; a handle of another kind or none
  * CUTT_INVALID_PLAN.  Inputs and outputs must not overlap (equal addresses are refused).

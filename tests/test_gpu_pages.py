@@ -2,6 +2,7 @@
 numbers and moved bytes, so everything is compared exactly."""
 import pytest
 
+from test_gpu_rows import few_sms  # noqa: F401 (a fixture)
 from test_rows_host import plain_build
 
 pytestmark = pytest.mark.gpu
@@ -94,6 +95,22 @@ def test_build_of_long_steps(native, b, m, in_place):
     if not in_place:
         assert c.torch.equal(c.pool, before)
         c.pool = out
+    c.check(want)
+
+
+@pytest.mark.parametrize("m", [3000, 16384, 20000])
+def test_build_in_place_in_a_context_of_few_sms(native, few_sms, m):  # noqa: F811
+    b, page = 5, 16
+    added = [m // b] * b
+    width = -(-added[0] // page) + 2
+    c = Build(native, [0, 3, 16, 17, 40], added, page, width, list(range(5000, 5000 + b * width)), [2, b * width], m)
+    c.plan = native.PagePlan(b, page, width, m, stream=few_sms)
+    if 8192 < m <= 16384:
+        assert '"cluster": 8' in c.plan.describe()
+    want = c.want()
+    c.torch.cuda.synchronize()
+    c.build()
+    c.torch.cuda.synchronize()
     c.check(want)
 
 

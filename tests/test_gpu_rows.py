@@ -710,6 +710,41 @@ def test_sorts_of_several_sizes_in_one_graph(native, order):
         r.check_map()
 
 
+@pytest.fixture
+def few_sms():
+    """A stream whose context has 16 SMs, which cannot hold a cluster of 16 blocks."""
+    import torch
+    d = pytest.importorskip("cuda.bindings.driver")
+    torch.zeros(1, device="cuda")
+
+    def ok(r):
+        assert int(r[0]) == 0, r
+        return r[1] if len(r) == 2 else r[1:]
+
+    dev = ok(d.cuDeviceGet(torch.cuda.current_device()))
+    sms = ok(d.cuDeviceGetDevResource(dev, d.CUdevResourceType.CU_DEV_RESOURCE_TYPE_SM))
+    parts = ok(d.cuDevSmResourceSplitByCount(1, sms, 0, 16))[0]
+    context = ok(d.cuGreenCtxCreate(ok(d.cuDevResourceGenerateDesc(parts[:1], 1)), dev, d.CUgreenCtxCreate_flags.CU_GREEN_CTX_DEFAULT_STREAM))
+    stream = ok(d.cuGreenCtxStreamCreate(context, d.CUstream_flags.CU_STREAM_NON_BLOCKING, 0))
+    yield int(stream)
+    torch.cuda.synchronize()
+    d.cuStreamDestroy(stream)
+    d.cuGreenCtxDestroy(context)
+
+
+@pytest.mark.parametrize("t,k,e", [(1024, 8, 64), (8192, 8, 256), (257, 10, 4096), (70001, 3, 129)])
+def test_map_in_a_context_of_few_sms(native, few_sms, t, k, e):
+    import torch
+    r = Run(native, routing(t, k, e, 6, 0.1), 8, "bf16", e, align=8)
+    r.plan = native.RowPlan(t, k, e, 8, r.code, align=8, stream=few_sms)
+    if 2048 < t * k <= 65536:
+        assert '"cluster": 8' in r.plan.describe()
+    torch.cuda.synchronize()
+    r.sort()
+    torch.cuda.synchronize()
+    r.check_map()
+
+
 def test_calls_on_another_device_are_refused(native):
     import torch
     if torch.cuda.device_count() < 2:

@@ -293,6 +293,22 @@ def test_local_expert(hc):
         assert f(e, 4, 3) == -1
 
 
+@pytest.mark.parametrize("most", [8, 16])
+def test_launch_of_the_map_fits_any_cluster(hc, most):
+    """Every number of slots is covered, in clusters of at most `most` blocks, within a block's shared memory, and a
+    block's ranks fit their bits."""
+    out = (ctypes.c_int * 4)()
+    for experts in (1, 7, 64, 256, 384, 1024, 2047, 4096):
+        for n in (0, 1, 31, 32, 33, 512, 513, 1024, 1025, 2048, 2049, 4096, 8191, 30000, 65535, 65536):
+            hc.cutt_hostcheck_sort_shape(n, experts, most, out)
+            blocks, slots, warps, words = out
+            assert 1 <= blocks <= most and blocks & (blocks - 1) == 0 and 1 <= warps <= 16
+            assert blocks * slots >= n and slots % 32 == 0 and slots < 1 << 19
+            assert words == 2 * slots + (2 * warps + 2) * experts + 3 * experts and words * 4 <= 216 * 1024
+    hc.cutt_hostcheck_sort_shape(65537, 4096, most, out)
+    assert out[0] == 0                                       # three kernels
+
+
 @pytest.mark.parametrize("elt", [1, 2, 4, 8])
 @pytest.mark.parametrize("heads,size,page,head_major,pad,shift", [
     (8, 128, 16, True, 0, 0), (1, 64, 1, False, 0, 0), (3, 33, 24, True, 0, 1), (2, 80, 64, False, 5, 0), (5, 1, 7, True, 1, 0),
