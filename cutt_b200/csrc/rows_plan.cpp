@@ -7,6 +7,18 @@ namespace {
 constexpr int kBad = 2;   // CUTT_INVALID_PARAMETER
 
 bool aligned(const void* p, size_t n) { return (uintptr_t)p % n == 0; }
+
+// Whether an output is given twice, or as an input too.  Null pointers are no addresses.
+bool shares(const void* const* out, int outs, const void* const* in, int ins) {
+  for (int i = 0; i < outs; i++) {
+    if (!out[i]) continue;
+    for (int j = 0; j < i; j++)
+      if (out[i] == out[j]) return true;
+    for (int j = 0; j < ins; j++)
+      if (out[i] == in[j]) return true;
+  }
+  return false;
+}
 }  // namespace
 
 int rows_element_bytes(int type) {
@@ -103,9 +115,11 @@ int check_rows_move(const RowsShape& s, const RowsMoveArgs& a) {
   if (a.needMap && (!a.count || !a.offset)) return kBad;
   if (s.type == 0 && (a.weight || a.dweight || !a.rowsOut)) return kBad;
   if ((a.dweight != nullptr) != (a.other != nullptr)) return kBad;
-  if (a.weight && a.weight == a.dweight) return kBad;
-  const void* out = a.rowsOut ? a.row : a.token;
-  if (a.other && a.other == out) return kBad;
+  // (tensors of no tokens are empty: their addresses mean nothing)
+  const void* out[] = {a.rowsOut ? a.row : slots ? a.token : nullptr, slots ? a.dweight : nullptr};
+  const void* in[] = {a.rowsOut ? slots ? a.token : nullptr : a.row, slots ? a.rowOf : nullptr, a.count, a.offset,
+                      slots ? a.weight : nullptr, slots || a.rowsOut ? a.other : nullptr};
+  if (shares(out, 2, in, 6)) return kBad;
   if (!aligned(a.token, elt) || !aligned(a.row, elt) || !aligned(a.other, elt)) return kBad;
   if (!aligned(a.rowOf, 4) || !aligned(a.count, 4) || !aligned(a.offset, 4) || !aligned(a.weight, 4) ||
       !aligned(a.dweight, 4))
@@ -147,8 +161,9 @@ int check_paged_move(const PagedShape& s, const void* k, const void* v, long lon
                      long long headStride, const void* slot, const void* kCache, const void* vCache,
                      bool rowsOut) {
   if (!k || !kCache || !slot || (v != nullptr) != (vCache != nullptr)) return kBad;
-  if (k == kCache || (v && (v == vCache || v == kCache || k == vCache))) return kBad;
-  if (v && (rowsOut ? k == v : kCache == vCache)) return kBad;
+  const void* rows[] = {k, v, s.tokens ? slot : nullptr};
+  const void* caches[] = {kCache, vCache, s.tokens ? slot : nullptr};
+  if (rowsOut ? shares(rows, 2, caches, 3) : shares(caches, 2, rows, 3)) return kBad;
   const void* p[] = {k, v, kCache, vCache};
   for (const void* q : p)
     if (!aligned(q, s.elt)) return kBad;

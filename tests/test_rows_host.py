@@ -160,6 +160,38 @@ def test_move_refusals(hc):
     assert rc(_ints(0, 2, 8, 0, 1, 8, 16, 2), token=0, rowOf=0) == 0
 
 
+@pytest.mark.parametrize("rows_out", [0, 1])
+def test_moves_refuse_an_output_that_is_also_given_elsewhere(hc, rows_out):
+    f = hc.cutt_hostcheck_rows_move
+    shape = _ints(4, 2, 8, 0, 1, 8, 16, 2)
+    names = ["token", "tokenStride", "row", "rowStride", "rowOf", "count", "offset", "weight", "other", "otherStride", "dweight", "rowsOut"]
+    good = dict(zip(names, [64, 16, 128, 16, 192, 256, 320, 384, 448, 16, 512, rows_out]))
+    pointers = ["token", "row", "rowOf", "count", "offset", "weight", "other", "dweight"]
+    assert f(shape, *good.values()) == 0
+    outputs = {"row" if rows_out else "token", "dweight"}
+    for out in outputs:
+        for name in pointers:
+            if name != out:
+                assert f(shape, *dict(good, **{out: good[name]}).values()) == BAD, (out, name)
+    inputs = [n for n in pointers if n not in outputs and n not in ("token", "row")]
+    for a in inputs:                                  # inputs may be shared
+        for b in inputs:
+            assert f(shape, *dict(good, **{a: good[b]}).values()) == 0, (a, b)
+
+
+def test_paged_moves_refuse_an_output_that_is_also_given_elsewhere(hc):
+    f = hc.cutt_hostcheck_paged_move
+    shape, strides = _ints(4, 2, 16, 2, 3, 8), (ctypes.c_longlong * 3)(256, 32, 16)
+    names = ["k", "v", "tokenStride", "headStride", "slot", "kCache", "vCache", "rowsOut"]
+    for rows_out, outputs in ((0, ("kCache", "vCache")), (1, ("k", "v"))):
+        good = dict(zip(names, [64, 128, 32, 16, 192, 256, 320, rows_out]))
+        assert f(shape, strides, *good.values()) == 0
+        for out in outputs:
+            for name in ("k", "v", "slot", "kCache", "vCache"):
+                if name != out:
+                    assert f(shape, strides, *dict(good, **{out: good[name]}).values()) == BAD, (out, name)
+
+
 def test_build_refusals(hc):
     f = hc.cutt_hostcheck_pages_build
     shape = _ints(4, 16, 8, 64)
