@@ -110,12 +110,11 @@ int check_rows_move(const RowsShape& s, const RowsMoveArgs& a) {
   const int elt = rows_element_bytes(s.type);
   const long long top = (1LL << 58) / elt;
   const long long slots = (long long)s.tokens * s.choices;
-  if (!a.row || a.token == a.row) return kBad;
-  if (slots && (!a.token || !a.rowOf)) return kBad;
+  // A plan of no tokens: its token-side tensors are empty, their addresses null or any.
+  if (!a.row || (slots && (!a.token || !a.rowOf || a.token == a.row))) return kBad;
   if (a.needMap && (!a.count || !a.offset)) return kBad;
   if (s.type == 0 && (a.weight || a.dweight || !a.rowsOut)) return kBad;
-  if ((a.dweight != nullptr) != (a.other != nullptr)) return kBad;
-  // (tensors of no tokens are empty: their addresses mean nothing)
+  if (slots && (a.dweight != nullptr) != (a.other != nullptr)) return kBad;
   const void* out[] = {a.rowsOut ? a.row : slots ? a.token : nullptr, slots ? a.dweight : nullptr};
   const void* in[] = {a.rowsOut ? slots ? a.token : nullptr : a.row, slots ? a.rowOf : nullptr, a.count, a.offset,
                       slots ? a.weight : nullptr, slots || a.rowsOut ? a.other : nullptr};
@@ -160,10 +159,12 @@ int check_pages_build(const PagesShape& s, const void* held, const void* added, 
 int check_paged_move(const PagedShape& s, const void* k, const void* v, long long tokenStride,
                      long long headStride, const void* slot, const void* kCache, const void* vCache,
                      bool rowsOut) {
-  if (!k || !kCache || !slot || (v != nullptr) != (vCache != nullptr)) return kBad;
-  const void* rows[] = {k, v, s.tokens ? slot : nullptr};
-  const void* caches[] = {kCache, vCache, s.tokens ? slot : nullptr};
-  if (rowsOut ? shares(rows, 2, caches, 3) : shares(caches, 2, rows, 3)) return kBad;
+  if (!kCache) return kBad;
+  // (rows and slots of no tokens are empty: their addresses are null or any)
+  if (s.tokens && (!k || !slot || (v != nullptr) != (vCache != nullptr))) return kBad;
+  const void* rows[] = {k, v, slot};
+  const void* caches[] = {kCache, vCache, slot};
+  if (s.tokens && (rowsOut ? shares(rows, 2, caches, 3) : shares(caches, 2, rows, 3))) return kBad;
   const void* p[] = {k, v, kCache, vCache};
   for (const void* q : p)
     if (!aligned(q, s.elt)) return kBad;

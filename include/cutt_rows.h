@@ -43,7 +43,8 @@ extern "C" {
  * token * choices + j names one choice.  This process holds experts firstExpert ..
  * firstExpert + experts - 1 (1 <= experts <= 4096); slots that name any other number are dropped.
  * `capacity` rows hold the sorted rows; each expert's segment starts at a multiple of `align`
- * (1 .. 4096).  tokens * choices and capacity are at most 2^30, width at most 2^24. */
+ * (1 .. 4096).  tokens * choices and capacity are at most 2^30, width at most 2^24.  With no tokens the
+ * tensors of tokens and slots are empty and may be NULL. */
 int cutt_rows_plan(unsigned int* handle, int tokens, int choices, int experts, int firstExpert,
                    int align, int capacity, int width, int type, void* stream);
 
@@ -87,8 +88,8 @@ int cutt_rows_combine_grad(unsigned int handle, const void* dout, long long dout
                            const int* count, const int* offset, const float* weight, const void* y,
                            long long yStride, void* dy, long long dyStride, float* dweight);
 
-/* Plan for block tables of `requests` rows of `tableWidth` pages each (requests * tableWidth <
- * 2^30) and slot maps of `maxTokens` entries (<= 2^30).  A page holds `pageSize` tokens. */
+/* Plan for block tables of `requests` rows (1 at least) of `tableWidth` pages each (requests *
+ * tableWidth < 2^30) and slot maps of `maxTokens` entries (<= 2^30).  A page holds `pageSize` tokens. */
 int cutt_pages_plan(unsigned int* handle, int requests, int pageSize, int tableWidth, int maxTokens,
                     void* stream);
 
@@ -113,7 +114,8 @@ int cutt_pages_build(unsigned int handle, const int* held, const int* added, con
 /* Plan for rows of `tokens` tokens x `heads` x `headSize` elements of sizeofType (1, 2, 4 or 8)
  * bytes in caches of `pages` pages of `pageSize` tokens: element d of head h of slot s lies at
  * (s / pageSize) * pageStride + (s % pageSize) * slotStride + h * headStride + d (strides in
- * elements, slotStride and headStride at least headSize). */
+ * elements, slotStride and headStride at least headSize).  With no tokens k, v and slot are empty and
+ * may be NULL. */
 int cutt_pages_plan_rows(unsigned int* handle, int tokens, int heads, int headSize, size_t sizeofType,
                          int pages, int pageSize, long long pageStride, long long slotStride,
                          long long headStride, void* stream);

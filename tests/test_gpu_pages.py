@@ -264,6 +264,18 @@ def test_one_row_to_many_slots_and_no_tokens(native):
     assert flat.abs().sum((1, 2)).count_nonzero() == 3
 
 
+def test_no_tokens_as_empty_tensors(native):
+    import torch
+    caches = [torch.ones(4, 8, 2, 16, device="cuda") for _ in range(2)]
+    row, slot = torch.zeros(0, 2, 16, device="cuda"), torch.zeros(0, dtype=torch.int64, device="cuda")
+    assert row.data_ptr() == 0 and slot.data_ptr() == 0
+    p = native.PagedRows(0, 2, 16, 4, 4, 8, 256, 32, 16)
+    p.store(row.data_ptr(), row.data_ptr(), slot.data_ptr(), *[c.data_ptr() for c in caches])
+    p.load(*[c.data_ptr() for c in caches], slot.data_ptr(), row.data_ptr(), row.data_ptr())
+    torch.cuda.synchronize()
+    assert all((c == 1).all() for c in caches)
+
+
 def test_cache_offsets_beyond_32_bits(native):
     """A cache of more than 2^32 bytes: the last pages hold what was stored there."""
     import torch

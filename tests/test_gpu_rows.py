@@ -155,6 +155,22 @@ def test_map_one_expert_for_all_and_long_ones(native, t, k, e):
     r.check_map()
 
 
+def test_calls_of_no_tokens(native):
+    """A step without tokens: empty tensors (null addresses); the calls succeed, rows keep what they hold."""
+    import torch
+    r = Run(native, torch.zeros(0, 2, dtype=torch.int64), 16, "f32", 4, align=8, capacity=16)
+    x, w = torch.zeros(0, 16, device="cuda"), torch.zeros(0, 2, device="cuda")
+    y, dy = torch.ones(16, 16, device="cuda"), torch.full((16, 16), 77.0, device="cuda")
+    assert x.data_ptr() == 0
+    r.sort()
+    r.plan.dispatch(x.data_ptr(), *r.maps(), dy.data_ptr(), weight=w.data_ptr())
+    r.plan.combine(y.data_ptr(), r.row_of.data_ptr(), x.data_ptr(), weight=w.data_ptr())
+    r.plan.combine_grad(x.data_ptr(), *r.maps(), dy.data_ptr(), weight=w.data_ptr(), y=y.data_ptr(), dweight=w.data_ptr())
+    r.plan.dispatch_grad(y.data_ptr(), r.row_of.data_ptr(), x.data_ptr(), weight=w.data_ptr(), x=x.data_ptr(), dweight=w.data_ptr())
+    r.check_map()
+    assert (dy == 77).all() and (y == 1).all()            # no segment has rows, so none is padded
+
+
 SHAPES = [  # tokens, choices, experts, width, align, pad, shift, drop
     (1, 8, 16, 512, 1, 0, 0, 0.0), (5, 1, 3, 1, 1, 0, 0, 0.0), (48, 6, 64, 2048, 1, 8, 0, 0.0), (33, 3, 7, 1111, 1, 0, 0, 0.2),
     (64, 4, 16, 264, 16, 0, 1, 0.2), (17, 10, 12, 136, 128, 24, 0, 0.3), (300, 2, 8, 40, 8, 3, 0, 0.9), (6000, 5, 24, 72, 8, 0, 0, 0.1),

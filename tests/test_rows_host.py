@@ -192,6 +192,24 @@ def test_paged_moves_refuse_an_output_that_is_also_given_elsewhere(hc):
                     assert f(shape, strides, *dict(good, **{out: good[name]}).values()) == BAD, (out, name)
 
 
+def test_calls_of_no_tokens_take_empty_tensors(hc):
+    """An empty tensor has the null address; the row side and the caches are there all the same."""
+    f = hc.cutt_hostcheck_rows_move
+    empty = _ints(0, 2, 8, 0, 4, 8, 16, 2)
+    # dispatch; the gradient of combine with the weights' gradient; combine; the gradient of dispatch
+    assert f(empty, 0, 16, 128, 16, 0, 256, 320, 0, 0, 0, 0, 1) == 0
+    assert f(empty, 0, 16, 128, 16, 0, 256, 320, 0, 512, 16, 0, 1) == 0
+    assert f(empty, 0, 16, 0, 16, 0, 256, 320, 0, 0, 0, 0, 1) == BAD         # the rows are written
+    assert f(empty, 0, 16, 128, 16, 0, 0, 320, 0, 0, 0, 0, 1) == BAD
+    g = hc.cutt_hostcheck_paged_move
+    shape, strides = _ints(0, 2, 16, 2, 3, 8), (ctypes.c_longlong * 3)(256, 32, 16)
+    for rows_out in (0, 1):
+        assert g(shape, strides, 0, 0, 32, 16, 0, 256, 320, rows_out) == 0
+        assert g(shape, strides, 0, 0, 32, 16, 0, 256, 0, rows_out) == 0
+        assert g(shape, strides, 0, 0, 32, 16, 0, 0, 320, rows_out) == BAD
+        assert g(shape, strides, 0, 0, 15, 16, 0, 256, 320, 1) == BAD
+
+
 def test_build_refusals(hc):
     f = hc.cutt_hostcheck_pages_build
     shape = _ints(4, 16, 8, 64)
