@@ -48,34 +48,64 @@ int cutt_hostcheck_paged_move(const int* shape, const long long* strides, const 
   return check_paged_move(s, k, v, tokenStride, headStride, slot, kCache, vCache, rowsOut != 0);
 }
 
-// cutt_pages_build on host arrays: the scan in a loop, then the kernel's expressions per token and
-// per page.  Returns the number of accesses outside the arrays (table: requests * tableStride
+// Exclusive prefix sums of a block's (tokens, pages) in the steps of the kernel's scan: within warps of 32, over the
+// warps' sums, then both together.
+struct Pair {
+  uint32_t tokens, pages;
+};
+static Pair operator+(Pair a, Pair b) { return Pair{add_up_to_int(a.tokens, b.tokens), a.pages + b.pages}; }
+static void warp_scan(Pair* x) {         // inclusive
+  for (int d = 1; d < 32; d <<= 1)
+    for (int lane = 31; lane >= d; lane--) x[lane] = x[lane] + x[lane - d];
+}
+static Pair block_scan(Pair* x, int threads) {
+  Pair sums[32] = {};
+  for (int w = 0; w < threads / 32; w++) {
+    warp_scan(x + w * 32);
+    sums[w] = x[w * 32 + 31];
+  }
+  warp_scan(sums);
+  for (int t = threads - 1; t >= 0; t--) {
+    const Pair inWarp = t % 32 ? x[t - 1] : Pair{0, 0};
+    x[t] = t / 32 ? inWarp + sums[t / 32 - 1] : inWarp;
+  }
+  return sums[threads / 32 - 1];
+}
+
+// cutt_pages_build on host arrays: the scan in blocks of `threads` requests, then the kernel's expressions per token
+// and per page.  Returns the number of accesses outside the arrays (table: requests * tableStride
 // entries, freeList: freeEntries), which are skipped.
-long long cutt_hostcheck_pages_run(int requests, int pageSize, int tableWidth, int maxTokens, const int* held, const int* added,
-                                   const int* freeList, int freeEntries, const int* poolIn, int* poolOut, int* table,
-                                   long long tableStride, int* tokenOffset, int* pageOffset, long long* slot) {
+static long long pages_run(int requests, int pageSize, int tableWidth, int maxTokens, const int* held, const int* added,
+                           const int* freeList, int freeEntries, const int* poolIn, int* poolOut, int* table,
+                           long long tableStride, int* tokenOffset, int* pageOffset, long long* slot, int threads) {
   PagesBuild p{PagesShape{requests, pageSize, tableWidth, maxTokens, make_fastdiv(pageSize)}, held, added, freeList, poolOut,
                table, tableStride, tokenOffset, pageOffset, slot};
-  long long tokens = 0, pages = 0, bad = 0;
+  long long bad = 0;
   int first = 0, limit = 0;
   if (freeList) {
     first = clamp_pool(poolIn[0]);
     limit = clamp_pool(poolIn[1]);
-    pages = first;
   }
-  for (int b = 0; b < requests; b++) {
-    tokenOffset[b] = saturate(tokens);
-    tokens += added[b] > 0 ? added[b] : 0;
-    if (freeList) {
-      pageOffset[b] = (int)pages;
-      pages += pages_taken(held[b], added[b], p.s.divPage, tableWidth);
+  Pair at{0, (uint32_t)first}, x[1024];
+  for (int b0 = 0; b0 < requests; b0 += threads) {
+    for (int t = 0; t < threads; t++) {
+      const int b = b0 + t;
+      const int n = b < requests && added[b] > 0 ? added[b] : 0;
+      x[t] = Pair{(uint32_t)n, b < requests && freeList ? (uint32_t)pages_taken(held[b], n, p.s.divPage, tableWidth) : 0u};
     }
+    const Pair total = block_scan(x, threads);
+    for (int t = 0; t < threads && b0 + t < requests; t++) {
+      const Pair q = at + x[t];
+      tokenOffset[b0 + t] = (int)q.tokens;
+      if (freeList) pageOffset[b0 + t] = (int)q.pages;
+    }
+    at = at + total;
   }
-  tokenOffset[requests] = saturate(tokens);
+  tokenOffset[requests] = (int)at.tokens;
   if (freeList) {
-    if (pages > 0x7fffffffLL) bad++;
-    pageOffset[requests] = (int)pages;
-    poolOut[0] = (int)pages < (first > limit ? first : limit) ? (int)pages : (first > limit ? first : limit);
+    if (at.pages > 0x7fffffffu) bad++;
+    pageOffset[requests] = (int)at.pages;
+    poolOut[0] = (int)at.pages < (first > limit ? first : limit) ? (int)at.pages : (first > limit ? first : limit);
     poolOut[1] = poolIn[1];
     if (limit > freeEntries) return -1;
   }
@@ -95,6 +125,13 @@ long long cutt_hostcheck_pages_run(int requests, int pageSize, int tableWidth, i
       take_page(p, b, f, limit);
     }
   return bad;
+}
+
+long long cutt_hostcheck_pages_run(int requests, int pageSize, int tableWidth, int maxTokens, const int* held, const int* added,
+                                   const int* freeList, int freeEntries, const int* poolIn, int* poolOut, int* table,
+                                   long long tableStride, int* tokenOffset, int* pageOffset, long long* slot) {
+  return pages_run(requests, pageSize, tableWidth, maxTokens, held, added, freeList, freeEntries, poolIn, poolOut, table,
+                   tableStride, tokenOffset, pageOffset, slot, requests > 512 || maxTokens > 512 ? 1024 : 512);
 }
 
 // Element offset of a slot in a cache, -1 where it is not one of the cache's.

@@ -11,9 +11,6 @@ namespace {
 
 constexpr unsigned kFull = 0xffffffffu;
 
-// Sum of two counts that stops at 2^31 - 1.  Associative, so a scan with it is the saturated scan.
-__device__ __forceinline__ unsigned add_up_to_int(unsigned a, unsigned b) { return min(a + b, 0x7fffffffu); }
-
 // Exclusive prefix sums of (tokens, pages) over the block: tokens saturate, pages cannot overflow
 // (a table has fewer than 2^30 entries).
 __device__ __forceinline__ uint2 block_scan2(uint2 v, uint2* s, uint2& total) {

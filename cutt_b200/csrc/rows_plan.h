@@ -105,7 +105,11 @@ CUTT_HD int pages_taken(int held, int added, const FastDiv& divPage, int tableWi
   return want > have ? (int)(want - have) : 0;
 }
 
-CUTT_HD int saturate(long long v) { return v > 0x7fffffffLL ? 0x7fffffff : (int)v; }
+// Sum of two counts that stops at 2^31 - 1.  Associative, so a scan with it is the saturated scan.
+CUTT_HD uint32_t add_up_to_int(uint32_t a, uint32_t b) {
+  const uint32_t c = a + b;              // counts are at most 2^31 - 1 each
+  return c < 0x7fffffffu ? c : 0x7fffffffu;
+}
 CUTT_HD int clamp_pool(int v) { return v < 0 ? 0 : v > kRowsMaxCount ? kRowsMaxCount : v; }
 
 // First entry greater than q of an ascending array of n entries, less one: the last request that

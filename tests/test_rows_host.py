@@ -325,6 +325,20 @@ def test_block_tables_at_the_ends_of_the_ranges(hc):
     assert got[3] == [1 << 35]
 
 
+@pytest.mark.parametrize("b", [31, 32, 33, 513, 1024, 1025, 2500])
+def test_offsets_of_many_requests(hc, b):
+    """Scans over several warps and blocks, with sums that pass 2^31 - 1 at every place of a warp."""
+    rng = random.Random(b)
+    for scale in (5, 2**31 // b, 2**31 // 40, 2**31 - 1):
+        held = [rng.randint(0, 40) for _ in range(b)]
+        added = [rng.choice([0, rng.randint(0, scale), scale]) for _ in range(b)]
+        page, width, m = 16, 6, 700
+        free = list(range(9000, 9000 + 3 * b))
+        table = [[rng.randint(0, 99) for _ in range(width)] for _ in range(b)]
+        got = run_build(hc, held, added, page, width, free, [1, 3 * b], table, m)
+        assert got == tuple(plain_build(held, added, page, width, free, [1, 3 * b], table, m))
+
+
 def test_cache_offsets_and_bad_slots(hc):
     f = hc.cutt_hostcheck_cache_offset
     for pages, page, ps, ss in ((7, 16, 4096, 256), (3, 24, 24 * 100, 100), (1 << 20, 1 << 14, 1 << 20, 64), (5, 1, 9, 9)):
