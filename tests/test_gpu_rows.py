@@ -171,6 +171,46 @@ def test_calls_of_no_tokens(native):
     assert (dy == 77).all() and (y == 1).all()            # no segment has rows, so none is padded
 
 
+@pytest.mark.parametrize("n,e,wide", [(1300001, 256, False), (2500000, 4096, True), (1 << 24, 60, False), (1 << 30, 300, False)])
+def test_maps_up_to_the_limit(native, n, e, wide):
+    """Maps whose chunks take several waves of blocks, up to 2^30 slots.  Checked on the device: counts, segments, each
+    slot's row in its expert's segment, each row's slot the one that has it, and slots ascending in every segment -
+    which together leave one map."""
+    import torch
+    align = 1 if n == 1 << 30 else 16
+    capacity = n + e * (align - 1)
+    g = torch.Generator(device="cuda").manual_seed(e)
+    ids = torch.randint(0, e + 1, (n,), device="cuda", generator=g, dtype=torch.int64 if wide else torch.int32)   # e: dropped
+    i32 = dict(dtype=torch.int32, device="cuda")
+    count, offset = torch.full((e,), -7, **i32), torch.full((e + 1,), -7, **i32)
+    row_of, slot_of = torch.full((n,), -7, **i32), torch.full((capacity,), -7, **i32)
+    plan = native.RowPlan(n, 1, e, 8, native.CUTT_ROWS_BF16, align=align, capacity=capacity, stream=torch.cuda.current_stream().cuda_stream)
+    plan.sort(ids.data_ptr(), ids.element_size(), count.data_ptr(), offset.data_ptr(), row_of.data_ptr(), slot_of.data_ptr())
+    torch.cuda.synchronize()
+    step = 1 << 26
+    want = sum(torch.bincount(ids[a:a + step], minlength=e + 1) for a in range(0, n, step))[:e]
+    assert torch.equal(count.long(), want)
+    assert torch.equal(offset.long(), torch.cat([want.new_zeros(1), ((want + align - 1) // align * align).cumsum(0)]))
+    first, end = torch.cat([offset[:e], offset.new_full((1,), -1)]), torch.cat([offset[:e] + count, offset.new_zeros(1)])
+    for a in range(0, n, step):
+        expert, row = ids[a:a + step].long(), row_of[a:a + step]
+        live = expert < e
+        assert ((row == -1) | live).all() and ((row >= first[expert]) & ((row < end[expert]) | ~live)).all()
+        back = slot_of[row.clamp_min(0).long()]
+        assert ((back == torch.arange(a, a + row.numel(), **i32)) | ~live).all()
+        del expert, row, live, back
+    held = 0
+    for a in range(0, capacity, step):                # rows: a slot (ascending in its segment) or none
+        slot = slot_of[a:a + step + 1]
+        one, two = slot[:-1], slot[1:]
+        at = torch.arange(a + 1, a + slot.numel(), **i32)
+        starts = torch.isin(at, offset)
+        assert ((two == -1) | (one < two) | starts).all()
+        assert ((two == -1) | (one >= 0) | starts).all()
+        held += (slot_of[a:a + step] >= 0).sum().item()
+    assert held == want.sum().item()
+
+
 SHAPES = [  # tokens, choices, experts, width, align, pad, shift, drop
     (1, 8, 16, 512, 1, 0, 0, 0.0), (5, 1, 3, 1, 1, 0, 0, 0.0), (48, 6, 64, 2048, 1, 8, 0, 0.0), (33, 3, 7, 1111, 1, 0, 0, 0.2),
     (64, 4, 16, 264, 16, 0, 1, 0.2), (17, 10, 12, 136, 128, 24, 0, 0.3), (300, 2, 8, 40, 8, 3, 0, 0.9), (6000, 5, 24, 72, 8, 0, 0, 0.1),
@@ -318,6 +358,19 @@ def test_every_launch_shape(native, kind, t, k, h, shift):
     want = (ts[:, None, :] * w.double()[:, :, None])[ok].cpu()
     close(y[row[ok]], want, want.abs(), 1, kind)
     assert (y[r.want[1][-1]:] == 77).all() and (y[r.padding()] == 0).all()
+
+
+MANY = [  # more choices than a walk over the row takes at once (16 with the weights' gradient, 8 without)
+    (50, 17, 20, 2048, 1, 0, 0, 0.2), (1300, 17, 32, 33, 8, 0, 0, 0.1), (40, 33, 16, 1111, 1, 0, 1, 0.3), (9, 100, 64, 264, 16, 8, 0, 0.5),
+    (1500, 24, 48, 136, 1, 0, 0, 0.0), (3, 16, 16, 515, 1, 0, 0, 0.0)]
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("shape", MANY)
+def test_many_choices(native, kind, shape):
+    test_dispatch(native, kind, shape)
+    test_combine(native, kind, shape)
+    test_gradients(native, kind, shape)
 
 
 def test_broadcast_inputs(native):
@@ -494,6 +547,67 @@ def test_layer_forward_and_backward(native):
     direction = torch.randn(t, k, generator=g)
     slope = (loss_w(w + step * direction) - loss_w(w - step * direction)) / (2 * step)
     assert abs(slope - (dw.double() * direction.double()).sum().item()) <= t * h * (k + 4) * 2.0 ** -24 * big / step / 16
+
+
+def test_layer_gradients_element_by_element(native):
+    """Every output and gradient of a layer within the roundings of its own terms, against autograd in 64 bits and
+    against differences.  A result of n terms, each made by at most three roundings of 2^-24, has at most n more in
+    its sum: (n + 4) * 2^-24 times the sum of its terms' magnitudes."""
+    import torch
+    t, k, e, h = 29, 3, 5, 48
+    g = torch.Generator().manual_seed(8)
+    ids = routing(t, k, e, 21, 0.1)
+    x, w, scale = torch.randn(t, h, generator=g), torch.randn(t, k, generator=g), torch.randn(e, h, generator=g)
+    dout = torch.randn(t, h, generator=g)
+    layer = _layer(native, t, k, e, h, "f32", 8)
+    on = ids.int().cuda()
+
+    def run(x, w):
+        return layer.forward(x.cuda(), on, w.cuda(), scale.cuda()).double().cpu()
+
+    out = run(x, w)
+    dx, dw, dscale = [v.double().cpu() for v in layer.backward(dout.cuda(), w.cuda(), scale.cuda())]
+    ok = (ids >= 0).double()
+
+    def plain(x, w, scale):
+        return (x[:, None, :] * scale[ids.clamp_min(0)] * (w * ok)[:, :, None]).sum(1)
+
+    def gradients(x, w, scale, dout):
+        v = [a.double().clone().requires_grad_() for a in (x, w, scale)]
+        y = plain(*v)
+        y.backward(dout.double())
+        return [y.detach()] + [a.grad for a in v]
+
+    u = 2.0 ** -24 * 1.001
+    got, want = (out, dx, dw, dscale), gradients(x, w, scale, dout)
+    # of magnitudes alone, the formulas give the sums of the terms' magnitudes
+    size = gradients(x.abs(), w.abs(), scale.abs(), dout.abs())
+    terms = (k, k, h, t * k)
+    limits = [(n + 4) * u * s for n, s in zip(terms, size)]
+    for a, b, limit in zip(got, want, limits):
+        assert ((a - b).abs() <= limit).all()
+    # the limits would show a term that is left out: the last column of dw, the last choice of out and dx
+    column = dout[:, None, -1] * x[:, None, -1] * scale[ids.clamp_min(0), -1] * ok
+    assert (column.abs() > limits[2])[ok > 0].double().mean() > 0.95
+    short = w.clone()
+    short[:, -1] = 0
+    for a, b, limit in zip(gradients(x, short, scale, dout)[:2], want, limits):
+        assert ((a - b).abs() > limit)[ok[:, -1] > 0].double().mean() > 0.95
+    # differences of the operators' own forward pass, which is linear in x and in w
+    step = 2.0 ** -4
+
+    def magnitude(x, w):
+        return ((k + 4) * u * plain(x.abs().double(), w.abs().double(), scale.abs().double()) * dout.abs().double()).sum().item()
+
+    for which, grad, limit in ((0, dx, limits[1]), (1, dw, limits[2])):
+        base = (x, w)[which]
+        direction = torch.randn(base.shape, generator=g)
+        ends = [[x, w], [x, w]]
+        for i, sign in enumerate((1, -1)):
+            ends[i][which] = base + sign * step * direction
+        moved = ends[0][which].double() - ends[1][which].double()
+        difference = ((run(*ends[0]) - run(*ends[1])) * dout.double()).sum().item()
+        assert abs(difference - (grad * moved).sum().item()) <= magnitude(*ends[0]) + magnitude(*ends[1]) + (limit * moved.abs()).sum().item()
 
 
 def test_layer_captured_and_replayed_with_new_routing(native):
