@@ -185,10 +185,9 @@ struct PagedLaunch {
 // STORE is a template parameter: with a flag the loads of a thread are no longer in flight at once (204
 // instead of 165 us).
 // A row is read only once its slot is known to be one of the cache's: k and v may end before the tokens whose
-// slots are not.  A store looks up the slots of all its accesses first: one by one 256 K and V rows took 3.1
-// instead of 2.65 us in a graph; 65536 take 93.1 instead of 91.3 us (58 registers instead of 48), and for the
-// same reason loads look them up one by one (131072 rows 165 us; slots first 167).
-template <int VB, bool STORE>
+// slots are not.  FIRST: a thread looks up the slots of all its accesses before the first of them, else one by
+// one (which takes fewer registers); launch_paged says when.
+template <int VB, bool STORE, bool FIRST>
 __global__ void __launch_bounds__(kPagedThreads) paged_kernel(const __grid_constant__ PagedLaunch l) {
   typedef typename Raw<VB>::T R;
   begin_row_kernel();
@@ -199,7 +198,7 @@ __global__ void __launch_bounds__(kPagedThreads) paged_kernel(const __grid_const
   for (uint32_t i0 = threadIdx.x; i0 < items; i0 += kPagedThreads * kPagedItems) {
     R value[kPagedItems];
     R* to[kPagedItems];
-    if (STORE) {
+    if (FIRST) {
       PagedPlace place[kPagedItems];
       long long slot[kPagedItems];
 #pragma unroll
@@ -215,8 +214,8 @@ __global__ void __launch_bounds__(kPagedThreads) paged_kernel(const __grid_const
         long long row, cache;
         to[k] = nullptr;
         if (!paged_access(l.p, place[k], slot[k], row, cache)) continue;
-        value[k] = __ldcs((const R*)(src + row));
-        to[k] = (R*)(dst + cache);
+        value[k] = __ldcs((const R*)(src + (STORE ? row : cache)));
+        to[k] = (R*)(dst + (STORE ? cache : row));
       }
     } else {
 #pragma unroll
@@ -227,8 +226,8 @@ __global__ void __launch_bounds__(kPagedThreads) paged_kernel(const __grid_const
         const PagedPlace a = paged_place(l.p, q0, i);
         long long row, cache;
         if (!paged_access(l.p, a, l.m.slot[a.token], row, cache)) continue;
-        value[k] = __ldcs((const R*)(src + cache));
-        to[k] = (R*)(dst + row);
+        value[k] = __ldcs((const R*)(src + (STORE ? row : cache)));
+        to[k] = (R*)(dst + (STORE ? cache : row));
       }
     }
 #pragma unroll
@@ -237,19 +236,30 @@ __global__ void __launch_bounds__(kPagedThreads) paged_kernel(const __grid_const
   }
 }
 
+// Blocks for an SM up to which a store looks up its slots first: with few blocks the time is the chain of slot and
+// row, with many it is how many of them an SM holds (58 registers a thread instead of 48, with narrow accesses 50
+// instead of 40).  K and V rows, us in a graph, slots first and one by one:
+//   8 heads of 128 bf16       256 rows 2.5, 3.1    8192 rows 13.6, 13.8    65536 rows 87.0, 86.2
+//   8 heads of 33 bf16        256 rows 2.1, 2.5    2048 rows 6.6, 6.6      65536 rows 153, 139
+// 8192 and 2048 rows are the same number of blocks there, 4096.  Loads: 131072 rows 167, 165.
+constexpr int kFirstBlocks = 28;
+
 template <int VB>
-cudaError_t paged_typed(const PagedLaunch& l, cudaStream_t stream) {
+cudaError_t paged_typed(const PagedLaunch& l, int numSM, cudaStream_t stream) {
   const dim3 grid((unsigned)((l.p.s.tokens + l.p.perBlock - 1) / l.p.perBlock), l.m.tensors, 1);
-  return l.m.store ? launch_row_kernel(paged_kernel<VB, true>, grid, kPagedThreads, 0, 0, stream, l)
-                   : launch_row_kernel(paged_kernel<VB, false>, grid, kPagedThreads, 0, 0, stream, l);
+  if (!l.m.store) return launch_row_kernel(paged_kernel<VB, false, false>, grid, kPagedThreads, 0, 0, stream, l);
+  if ((long long)grid.x * grid.y <= (long long)kFirstBlocks * numSM)
+    return launch_row_kernel(paged_kernel<VB, true, true>, grid, kPagedThreads, 0, 0, stream, l);
+  return launch_row_kernel(paged_kernel<VB, true, false>, grid, kPagedThreads, 0, 0, stream, l);
 }
 
 }  // namespace
 
 // Tokens of a block.
 constexpr int kBlockTokens = 1024;
-// With the pool updated in place: up to this many tokens a cluster, above two kernels.  Measured:
-// 8192 tokens 6.1 against 7.4 us, 131072 tokens 12.6 against 6.8 us.
+// With the pool updated in place: up to this many tokens a cluster, above two kernels.  Measured, 61 requests:
+// 8192 tokens 5.0 against 5.7 us, 16384 tokens 4.8 against 5.7, 32768 tokens 5.6 against 5.7, 131072 tokens 10.9
+// against 5.8; 256 requests with one token each 3.3 against 5.2.
 constexpr int kClusterTokens = 16384;
 
 // Blocks and threads of the one kernel.
@@ -281,17 +291,17 @@ cudaError_t launch_pages_build(const PagesBuild& b, const int* poolIn, int* pool
   return launch_row_kernel(pages_expand, dim3(want < 1 ? 1 : want < most ? want : most), kExpandThreads, 0, 0, stream, b);
 }
 
-cudaError_t launch_paged(const PagedShape& s, const PagedMove& m, cudaStream_t stream) {
+cudaError_t launch_paged(const PagedShape& s, const PagedMove& m, int numSM, cudaStream_t stream) {
   if (s.tokens == 0) return cudaSuccess;
   unsigned long long addresses = 0;
   for (int i = 0; i < m.tensors; i++) addresses |= (uintptr_t)m.src[i] | (uintptr_t)m.dst[i];
   const PagedLaunch l{paged_items(s, m.tokenStride, m.headStride, addresses), m};
   switch (l.p.access) {
-    case 16: return paged_typed<16>(l, stream);
-    case 8: return paged_typed<8>(l, stream);
-    case 4: return paged_typed<4>(l, stream);
-    case 2: return paged_typed<2>(l, stream);
-    default: return paged_typed<1>(l, stream);
+    case 16: return paged_typed<16>(l, numSM, stream);
+    case 8: return paged_typed<8>(l, numSM, stream);
+    case 4: return paged_typed<4>(l, numSM, stream);
+    case 2: return paged_typed<2>(l, numSM, stream);
+    default: return paged_typed<1>(l, numSM, stream);
   }
 }
 

@@ -115,7 +115,7 @@ struct PagedMove {
   int tensors;                         // 1 or 2
   int store;                           // rows to cache, else cache to rows
 };
-cudaError_t launch_paged(const PagedShape& s, const PagedMove& m, cudaStream_t stream);
+cudaError_t launch_paged(const PagedShape& s, const PagedMove& m, int numSM, cudaStream_t stream);
 
 // Row plans of the public handle space (rows_api.cu).  Their numbers have the top bit set, which
 // cuttPlan's never reach.

@@ -238,7 +238,7 @@ static int move_paged(unsigned int handle, const void* k, const void* v, long lo
   m.headStride = headStride * s.elt;
   m.slot = slot;
   m.store = store ? 1 : 0;
-  return result(launch_paged(s, m, p->stream));
+  return result(launch_paged(s, m, p->numSM, p->stream));
 }
 
 int cutt_pages_store(unsigned int handle, const void* k, const void* v, long long tokenStride, long long headStride,

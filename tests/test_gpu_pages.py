@@ -229,6 +229,32 @@ def test_store_and_load(native, elt, heads, size, page, head_major, pad):
         k, v = v, k
 
 
+@pytest.mark.parametrize("elt,heads,size", [(2, 8, 128), (2, 8, 36), (4, 8, 33), (2, 8, 33), (1, 9, 57)])      # 16, 8, 4, 2, 1 bytes
+@pytest.mark.parametrize("have", [9000, 8111])
+def test_store_of_many_rows(native, elt, heads, size, have):
+    """Stores of more blocks than the device holds at once, with slots that are none and rows that end early."""
+    import torch
+    dt = {1: torch.uint8, 2: torch.int16, 4: torch.int32}[elt]
+    n, page = 9000, 16
+    pages = -(-n // page) + 3
+    g = torch.Generator(device="cuda").manual_seed(size)
+    rand = lambda *s: torch.randint(0, 200, s, device="cuda", generator=g, dtype=dt)
+    caches = [rand(pages, heads, page, size) for _ in range(2)]
+    rows = [rand(have, heads, size) for _ in range(2)]
+    slot = torch.randperm(pages * page, device="cuda", generator=g)[:n]
+    slot[::11] = -1
+    slot[have:] = pages * page
+    slot = slot.contiguous()
+    ok = slot[:have] >= 0
+    want = [c.clone() for c in caches]
+    for w, r in zip(want, rows):
+        w.transpose(1, 2)[slot[:have][ok] // page, slot[:have][ok] % page] = r[ok]
+    p = native.PagedRows(n, heads, size, elt, pages, page, heads * page * size, size, page * size,
+                         stream=torch.cuda.current_stream().cuda_stream)
+    p.store(rows[0].data_ptr(), rows[1].data_ptr(), slot.data_ptr(), caches[0].data_ptr(), caches[1].data_ptr())
+    assert torch.equal(caches[0], want[0]) and torch.equal(caches[1], want[1])
+
+
 @pytest.mark.parametrize("size", [64, 33])
 def test_rows_end_before_skipped_tokens(native, size):
     """A batch shorter than the plan's tokens: the slots behind its last row are -1."""
