@@ -186,7 +186,7 @@ struct PagedLaunch {
 // instead of 165 us).
 // A row is read only once its slot is known to be one of the cache's: k and v may end before the tokens whose
 // slots are not.  FIRST: a thread looks up the slots of all its accesses before the first of them, else one by
-// one (which takes fewer registers); launch_paged says when.
+// one (which takes fewer registers); kFirstBlocks says when.
 template <int VB, bool STORE, bool FIRST>
 __global__ void __launch_bounds__(kPagedThreads) paged_kernel(const __grid_constant__ PagedLaunch l) {
   typedef typename Raw<VB>::T R;

@@ -3,9 +3,14 @@
 // dispatch), with the gradient of the weights on the way.
 //
 // Both walk over tokens, so the token side is read or written once and the k-fold side once: the
-// fewest bytes there are.  A block owns a token, or a part of its row; every thread holds one access
-// of the token's row and goes through the token's slots.  Sums are in 32 bits in the order of the
-// slots, rounded once, so results do not depend on the launch shape.
+// fewest bytes there are.  (From memory: a token's row is read again for each four or eight of its slots,
+// which finds it in the cache, and with more than 16 choices sums with the weights' gradient take a walk
+// over the rows for the gradient and one for the sums.)  A block owns a token, or a part of its row; every
+// thread holds one access of the token's row and goes through the token's slots.  Sums over slots are in
+// 32 bits in the order of the slots, rounded once, so they do not depend on the launch shape.  The weights'
+// gradients are sums along the row, made by a block's threads together: their order, and with it the last
+// bits, depends on the number of threads, which is chosen from the tokens, the row's length and the SMs, and
+// on the alignment of the rows.  The same call gives the same bits.
 //
 // What bounds them is memory: 16384 tokens to 8 rows of 8 KB (bf16) take 188 us, 6.4 TB/s, which is
 // what a copy reaches.  Blocks of one token that end soon, many of them on an SM, do best: teams that
@@ -198,9 +203,10 @@ __device__ __forceinline__ bool near_rows(const RowsMove& m, const int (&row)[KU
 // with the weights' gradient (16384 tokens, half of 8 slots dropped, 4 KB) 24 warps 110, 32 warps 124;
 // 16384 tokens to 8 rows of 2001 bf16 with 32, 48, 64 warps 119, 126, 132; sums of 8 rows of 4 KB, half
 // dropped, 24, 28, 32 warps 60, 57, 59; sums of 4 rows of 5 KB 32, 40, 48 warps 36.2, 35.2, 35.5; sums of 10
-// rows of 4 KB with the weights' gradient 16, 20, 24 warps 171, 110, 139; of 3 rows of 1111 fp32 with it (1023
-// tokens) 32, 40 warps 8.4, 10.4.
-constexpr int scatter_warps(bool, bool dot) { return dot ? 24 : 32; }
+// rows of 4 KB with the weights' gradient 16, 20, 24 warps 171, 110, 139.  Sums of up to 4 rows with it, 32 and
+// 40 warps: 3 rows of 1111 fp32 (1023 tokens) 8.4, 10.4; of 1112 fp32 6.0, 6.1; of 1024 bf16 4.6, 4.8; 4 rows of 4096
+// bf16 (1024 tokens) 11.4, 11.8; of 2048 bf16 (16384 tokens) 64.9, 66.6; of 2048 fp32 (8192 tokens) 63.5, 64.0.
+constexpr int scatter_warps(bool dot) { return dot ? 24 : 32; }
 constexpr int gather_warps(int ku, bool dot) { return ku > 8 ? 20 : ku > 4 ? 28 : dot ? 32 : 40; }
 
 // ANY: rows at any address; the pieces of a row are then cut at the 16-byte boundaries of the row
@@ -211,7 +217,7 @@ constexpr int gather_warps(int ku, bool dot) { return ku > 8 ? 20 : ku > 4 ? 28 
 // grid.x: blocks of padding (experts * kPadBlocks of them, or none), then one for each token; grid.y:
 // parts of a row.
 template <typename T, bool ANY, int KU, int THREADS, bool WEIGHT, bool DOT>
-__global__ void __launch_bounds__(THREADS, scatter_warps(ANY, DOT) * 32 / THREADS)
+__global__ void __launch_bounds__(THREADS, scatter_warps(DOT) * 32 / THREADS)
 scatter_kernel(const __grid_constant__ RowsMove m, int padBlocks) {
   __shared__ float part[THREADS / 32][KU];
   begin_row_kernel();
@@ -440,21 +446,26 @@ gather_kernel(const __grid_constant__ RowsMove m) {
 }
 
 // Threads of a token's block.  Measured with 16384 tokens in bf16, us with 64, 128, 256 and 512 threads:
-//   to 8 rows of 8 KB      209, 200, 195, 188      to 2 rows of 8 KB      70,  70,  75,  98
-//   to 4 rows of 8 KB      110, 107, 107, 126      to 8 rows of 2 KB      51,  49,  49,  64
+//   to 8 rows of 8 KB      204, 199, 195, 192      to 2 rows of 8 KB      73, 74, 79, 93
+//   to 4 rows of 8 KB      118, 116, 114, 125      to 8 rows of 2 KB      55, 54, 54, 69
 // so a thread is to have at least 8 stores.  With weights it needs registers, and 512 threads took 201
 // where 256 took 193.
 int scatter_threads(long long pieces, bool weight) {
   if (pieces >= 8 * 512 && !weight) return 512;
   return pieces >= 8 * 256 ? 256 : pieces >= 8 * 128 ? 128 : 64;
 }
-// The gradient of the weights with it (64, 128, 256 threads): 8 rows of 8 KB 370, 360, 360; half of them
-// dropped 198, 197, 211; 8 rows of 4 KB 184, 179, 186; half dropped 100, 103, 119; 2 KB 92, 92, 121.  Sums: 8 rows of 8 KB 178, 174, 176; half of 8 rows
-// of 4 KB dropped 57, 61, 75; 8 rows of 2 KB 40, 44, 62.
+// With the weights' gradient, us with 64, 128 and 256 threads (bf16, 8 slots to a token):
+//                                        rows out (combine_grad)     sums (dispatch_grad)
+//   16384 tokens, rows of 8 KB             361, 354, 352               214, 209, 226
+//     half of the slots dropped            206, 207, 226               147, 145, 173
+//   16384 tokens, rows of 4 KB             193, 191, 195               116, 115, 135
+//     half of the slots dropped            106, 116, 135               77, 81, 109
+//   16384 tokens, rows of 2 KB             98, 100, 133                60, 65, 107
+//   1024 tokens, rows of 8 KB              28.3, 30.4, 27.3            21.0, 19.4, 20.1
+//   256 tokens, rows of 8 KB               14.8, 11.1, 9.8             13.7, 9.2, 7.4
 // Few tokens (less than 8 for an SM): without a sum along the row several blocks of 128 threads share
-// one.  With a sum one block has to make it, and more threads are better (256 tokens, 8 rows of 8 KB:
-// 16, 11.3, 9.7; 13.1, 9.0, 7.3; 1024 tokens 28.4, 28.9, 26.9; 19.1, 18.5, 17.8) unless blocks are
-// many and rows too short for them (1023 tokens, 3 rows of 1111 fp32, 128 threads 8.4, 256 11.0).
+// one.  With a sum one block has to make it, and more threads are better unless blocks are many and
+// rows too short for them (1023 tokens, 3 rows of 1111 fp32, sums with 128 threads 8.4, with 256 10.8).
 constexpr int kFewTokens = 8;            // for an SM
 constexpr int kMostParts = 8;
 

@@ -41,12 +41,12 @@ int check_rows_shape(const RowsShape& s) {
   return 0;
 }
 
-// Up to kClusterSlots slots a cluster, above three kernels.  Measured, 128 experts: 32768 slots 6.2
-// against 8.1 us, 65536 slots 7.5 against 8.3 us, and one launch against three; 524288 slots of 256
-// experts take 13 us in three kernels.
+// Up to kClusterSlots slots a cluster, above three kernels.  Measured, 128 experts: 32768 slots 5.5
+// against 7.8 us, 65536 slots 6.9 against 7.8 us, and one launch against three; 524288 slots of 256
+// experts and 64-bit indices take 12.5 us in three kernels.
 // A block takes this many slots where one is enough, else half of them, and more once the cluster is
-// full: 512 slots 4.4 us in one block, 4.2 in two; 288 slots 3.8 and 4.5; 1024 slots 4.6 in four, 5.2
-// in two.
+// full: 288 slots 3.3 us in one block and in four, 512 slots 3.7 and 3.5; 1024 slots 3.5 in four, 4.1
+// in one.
 constexpr int kBlockSlots = 512;
 
 int ranked_words(int slots, int warps, int experts) { return 2 * slots + (2 * warps + 2) * experts; }

@@ -69,8 +69,8 @@ constexpr int kClusterSlots = 65536;
 constexpr int kMostClusterBlocks = 16;
 constexpr int kPortableBlocks = 8;            // of a cluster that every device can hold
 constexpr int kMostSortWords = 216 * 1024 / 4;   // of a block's shared memory
-// Warps of a block: one for 32 slots, at most 16 (every further one is a histogram to clear and to scan:
-// 8192 slots per block with 32 warps instead of 16 took 8 us instead of 6).
+// Warps of a block: one for 32 slots, at most 16 (every further one is a histogram to clear and to scan).
+// 8, 16, 32 of them: 65536 slots of 128 experts 8.8, 6.9, 8.4 us; 524288 slots of 256 experts 13.4, 12.4, 14.7.
 constexpr int kSortWarps = 16;
 struct SortShape {
   int blocks, slots, warps;   // of the cluster, of a block, of a block

@@ -60,8 +60,10 @@ int cutt_rows_sort(unsigned int handle, const void* expertOf, size_t sizeofIndex
                    int* offset, int* rowOf, int* slotOf);
 
 /* Row strides below are in elements.  An input's may be anything from 0 (one row for all) up, an
- * output's is at least `width`.  weight[slots] may be NULL (1 everywhere).  Entries of rowOf
- * outside 0 .. capacity-1 are taken as dropped. */
+ * output's is at least `width`.  Token-side inputs have `tokens` rows, row-side ones `capacity`; all of
+ * them, and what lies between them, may be read.  weight[slots] may be NULL (1 everywhere).  Entries of
+ * rowOf outside 0 .. capacity-1 are taken as dropped.  Sums over slots are in the order of the slots;
+ * the last bits of dweight depend on the shapes, the strides' alignment and the device, not on the run. */
 
 /* y[rowOf[s]] = weight[s] * x[s / choices]; padding rows inside the segments (between
  * offset[e] + count[e] and offset[e+1]) become zero; rows from offset[experts] on are left alone. */

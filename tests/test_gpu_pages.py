@@ -229,7 +229,7 @@ def test_store_and_load(native, elt, heads, size, page, head_major, pad):
         k, v = v, k
 
 
-@pytest.mark.parametrize("elt,heads,size", [(2, 8, 128), (2, 8, 36), (4, 8, 33), (2, 8, 33), (1, 9, 57)])      # 16, 8, 4, 2, 1 bytes
+@pytest.mark.parametrize("elt,heads,size", [(2, 8, 128), (2, 16, 36), (4, 8, 33), (2, 8, 33), (1, 9, 57)])      # 16, 8, 4, 2, 1 bytes
 @pytest.mark.parametrize("have", [9000, 8111])
 def test_store_of_many_rows(native, elt, heads, size, have):
     """Stores of more blocks than the device holds at once, with slots that are none and rows that end early."""

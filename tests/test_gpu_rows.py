@@ -862,6 +862,24 @@ def few_sms():
     d.cuGreenCtxDestroy(context)
 
 
+def test_plans_made_while_their_stream_is_captured(native):
+    """A plan may be made inside a capture: it asks what its stream's context can hold, and launches nothing."""
+    import torch
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        r = Run(native, routing(1024, 8, 64, 1), 8, "bf16", 64, align=8)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        r.plan = native.RowPlan(1024, 8, 64, 8, r.code, align=8, stream=side.cuda_stream)
+        pages = native.PagePlan(4, 16, 1100, 16384, stream=side.cuda_stream)
+        r.sort()
+    assert '"cluster": 16' in r.plan.describe() and '"cluster": 16' in pages.describe()
+    graph.replay()
+    torch.cuda.synchronize()
+    r.check_map()
+
+
 @pytest.mark.parametrize("t,k,e", [(1024, 8, 64), (8192, 8, 256), (257, 10, 4096), (70001, 3, 129)])
 def test_map_in_a_context_of_few_sms(native, few_sms, t, k, e):
     import torch
